@@ -47,6 +47,13 @@ SIGNATURES = {
     "hk_lse_merge": (C.c_int, [P, P, I32, I64, I32, P, P, P]),
     "hk_sample_workspace_size": (SZ, [I32, I32]),
     "hk_sample_verify": (C.c_int, [P, I32, P, I32, I32, I32, P, P, P, I32, P, P, P, SZ, P]),
+    "hk_qk_norm_rope": (C.c_int, [P, I64, P, I64, P, P, P, I64, I32, I32, P, I32, I32, I32, I32, F32, I32, P, I64, P, I64, P]),
+    "hk_gqa_append_fp8": (C.c_int, [P, I64, P, I64, I32, P, I32, I32, I32, I32, I64, P, P, P, P, P, P, P]),
+    "hk_gqa_fp8_workspace_size": (SZ, [I32, I32, I32, I32]),
+    "hk_gqa_decode_fp8": (C.c_int, [P, I64, P, P, P, P, P, I32, P, P, I32, I32, I32, I32, I32, I32, I64, I32, I32, F32, I32, P, P, P, SZ, P]),
+    "hk_gqa_select_workspace_size": (SZ, [I32, I32, I32, I32]),
+    "hk_gqa_select_blocks": (C.c_int, [P, I64, P, P, P, I32, P, P, I32, I32, I32, I32, I32, I32, I64, I32, I32, I32, I32, I32, P, P, SZ, P]),
+    "hk_gqa_sparse_fp8": (C.c_int, [P, I64, P, P, P, P, P, I32, P, P, P, I32, I32, I32, I32, I32, I32, I32, I64, F32, I32, P, P, P, SZ, P]),
     "hk_quant_fp8": (C.c_int, [P, I64, I32, P, P, P]),
     "hk_gemm_fp8": (C.c_int, [P, P, P, P, I64, I32, I32, P, P]),
     "hk_route": (C.c_int, [P, P, I32, I32, I32, F32, P, P, P]),
@@ -318,6 +325,182 @@ def mla_partial(q, kv_cache, block_table, cu_seqlens, positions, kv_begin, kv_en
          kv_cache.shape[0], max_kv_len, scale, ptr(o), ptr(lse), ptr(workspace), workspace.numel(),
          stream_ptr(stream))
     return o, lse
+
+
+# ---- GQA over the block-scaled 8-bit cache -----------------------------------------------
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # HK_BF16, HK_F16
+
+
+def _rows(t, like=None):
+    """(address, row stride in elements) of a [rows, heads, dim] tensor whose rows may be slices of
+    wider ones; with `like`, also of its shape, type and device."""
+    T, h, d = t.shape
+    s = t.stride()
+    if like is not None and (t.shape, t.dtype, t.device) != (like.shape, like.dtype, like.device):
+        raise ValueError(f"expected a {like.dtype} tensor of shape {tuple(like.shape)} on {like.device}")
+    if T > 1 and h > 0:
+        if s[2] != 1 or (s[1] != d and h > 1):
+            raise ValueError("heads of a row must lie side by side")
+        return t.data_ptr(), s[0]
+    if h > 0 and (s[2] != 1 or (s[1] != d and h > 1)):
+        raise ValueError("heads of a row must lie side by side")
+    return t.data_ptr(), h * d
+
+
+def _here(dtype, *tensors):
+    """The HK_BF16 / HK_F16 code, after checking that every tensor is on the current device."""
+    if dtype not in _DTYPES:
+        raise TypeError(f"expected bfloat16 or float16, got {dtype}")
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+    return _DTYPES[dtype]
+
+
+def _typed(t, dtype, name):
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor")
+    return t.data_ptr()
+
+
+def qk_norm_rope(q, k, positions, table, q_gain=None, k_gain=None, interleaved=False, eps=1e-6,
+                 q_out=None, k_out=None, stream=None):
+    """RMS norm of each query and key head, then the rotation by table[positions] (fp32, the layout
+    of `rope_table`; its width is the number of rotated dims).  q [T, heads, dim] and k may be
+    slices of a fused projection; outputs are new contiguous tensors unless given (q_out=q works
+    in place).  Returns (q_out, k_out)."""
+    T, H, D = q.shape
+    G = k.shape[1]
+    if k.shape != (T, G, D) or k.dtype != q.dtype or positions.shape[0] < T or table.dim() != 2:
+        raise ValueError("q, k, positions and table do not fit together")
+    for w in (q_gain, k_gain):
+        if w is not None and w.shape != (D,):
+            raise ValueError(f"a gain has {D} elements")
+    dt = _here(q.dtype, q, k, positions, table, q_gain, k_gain, q_out, k_out)
+    if q_out is None:
+        q_out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    if k_out is None:
+        k_out = torch.empty((T, G, D), dtype=q.dtype, device=q.device)
+    (qp, qs), (kp, ks), (yp, ys), (zp, zs) = _rows(q), _rows(k), _rows(q_out, q), _rows(k_out, k)
+    call("hk_qk_norm_rope", qp, qs, kp, ks, _typed(q_gain, q.dtype, "q_gain"), _typed(k_gain, q.dtype, "k_gain"),
+         _typed(table, torch.float32, "table"), table.shape[0], table.shape[1], int(interleaved),
+         _typed(positions, torch.int32, "positions"), T, H, G, D, eps, dt, yp, ys, zp, zs, stream_ptr(stream))
+    return q_out, k_out
+
+
+def _gqa_cache(k_cache, v_cache, k_scale, v_scale):
+    """(pages, KV heads, page rows, dim) of a cache after checking its four arrays."""
+    N, G, R, D = k_cache.shape
+    if v_cache.shape != k_cache.shape or k_scale.shape != (N, G) or v_scale.shape != (N, G):
+        raise ValueError("k_cache, v_cache [pages, kv_heads, page, dim] and their scales [pages, kv_heads] do not fit together")
+    return N, G, R, D
+
+
+def gqa_append_fp8(k_new, v_new, slot_mapping, k_cache, v_cache, k_scale, v_scale, centroids=None,
+                   centroid_scale=None, stream=None):
+    """Appends rows to the block-scaled e4m3 cache (uint8 [pages, kv_heads, page, dim], fp32 scales
+    [pages, kv_heads]) and, when given, the int8 centroids of the pages that become full."""
+    N, G, R, D = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
+    T = k_new.shape[0]
+    if k_new.shape != (T, G, D) or v_new.shape != (T, G, D) or v_new.dtype != k_new.dtype or slot_mapping.shape[0] < T:
+        raise ValueError("k_new, v_new [rows, kv_heads, dim] and slot_mapping do not fit the cache")
+    if centroids is not None and (centroids.shape != (N, G, D) or centroid_scale is None or centroid_scale.shape != (N, G)):
+        raise ValueError("centroids [pages, kv_heads, dim] need centroid_scale [pages, kv_heads]")
+    dt = _here(k_new.dtype, k_new, v_new, slot_mapping, k_cache, v_cache, k_scale, v_scale, centroids, centroid_scale)
+    (kp, ks), (vp, vs) = _rows(k_new), _rows(v_new)
+    call("hk_gqa_append_fp8", kp, ks, vp, vs, dt, _typed(slot_mapping, torch.int32, "slot_mapping"), T, G, D, R, N,
+         _typed(k_cache, torch.uint8, "k_cache"), _typed(v_cache, torch.uint8, "v_cache"),
+         _typed(k_scale, torch.float32, "k_scale"), _typed(v_scale, torch.float32, "v_scale"),
+         _typed(centroids, torch.int8, "centroids"), _typed(centroid_scale, torch.float32, "centroid_scale"), stream_ptr(stream))
+
+
+def gqa_fp8_workspace_size(num_tokens, q_heads, kv_heads, head_dim) -> int:
+    return lib().hk_gqa_fp8_workspace_size(num_tokens, q_heads, kv_heads, head_dim)
+
+
+def _gqa_io(q, G, D, out, lse, workspace):
+    T, H, d = q.shape
+    if d != D:
+        raise ValueError(f"q has heads of {d} dims, the cache of {D}")
+    if out is None:
+        out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
+    if out.shape != q.shape or lse.shape != (T, H):
+        raise ValueError("out and lse do not fit q")
+    if workspace is None:
+        workspace = torch.empty(gqa_fp8_workspace_size(T, H, G, D), dtype=torch.uint8, device=q.device)
+    return out, lse, workspace
+
+
+def _lanes(block_table, cu_seqlens, positions, T):
+    if block_table.dim() != 2 or cu_seqlens.shape[0] != block_table.shape[0] + 1 or positions.shape[0] < T:
+        raise ValueError("block_table [lanes, pages], cu_seqlens [lanes + 1] and positions do not fit together")
+    return (_typed(block_table, torch.int32, "block_table"), block_table.shape[1],
+            _typed(cu_seqlens, torch.int32, "cu_seqlens"), _typed(positions, torch.int32, "positions"))
+
+
+def gqa_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, max_rows,
+                   max_kv_len, scale, out=None, lse=None, workspace=None, stream=None):
+    """Ragged paged attention over the block-scaled cache of `gqa_append_fp8`: every lane's rows
+    (at most max_rows) attend the lane's KV rows up to their positions.  Returns (out, lse)."""
+    N, G, R, D = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
+    T, H, _ = q.shape
+    dt = _here(q.dtype, q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, out, lse, workspace)
+    out, lse, workspace = _gqa_io(q, G, D, out, lse, workspace)
+    qp, qs = _rows(q)
+    bt, stride, cu, pos = _lanes(block_table, cu_seqlens, positions, T)
+    call("hk_gqa_decode_fp8", qp, qs, _typed(k_cache, torch.uint8, "k_cache"), _typed(v_cache, torch.uint8, "v_cache"),
+         _typed(k_scale, torch.float32, "k_scale"), _typed(v_scale, torch.float32, "v_scale"), bt, stride, cu, pos,
+         block_table.shape[0], T, H, G, D, R, N, max_rows, max_kv_len, scale, dt, _typed(out, q.dtype, "out"),
+         _typed(lse, torch.float32, "lse"), ptr(workspace), workspace.numel(), stream_ptr(stream))
+    return out, lse
+
+
+def gqa_select_blocks(q, centroids, centroid_scale, block_table, cu_seqlens, positions, page_size, max_kv_len,
+                      top_blocks, sink=1, local=1, blocks=None, workspace=None, stream=None):
+    """The blocks each row and KV head reads, by its int8 score against the pages' centroids:
+    int32 [T, kv_heads, top_blocks], rising, -1 behind the last."""
+    N, G, D = centroids.shape
+    T, H, d = q.shape
+    if d != D or centroid_scale.shape != (N, G):
+        raise ValueError("q, centroids and centroid_scale do not fit together")
+    dt = _here(q.dtype, q, centroids, centroid_scale, block_table, cu_seqlens, positions, blocks, workspace)
+    if blocks is None:
+        blocks = torch.empty((T, G, top_blocks), dtype=torch.int32, device=q.device)
+    elif blocks.shape != (T, G, top_blocks):
+        raise ValueError("blocks must be [T, kv_heads, top_blocks]")
+    if workspace is None:
+        workspace = torch.empty(lib().hk_gqa_select_workspace_size(T, G, page_size, max_kv_len), dtype=torch.uint8, device=q.device)
+    qp, qs = _rows(q)
+    bt, stride, cu, pos = _lanes(block_table, cu_seqlens, positions, T)
+    call("hk_gqa_select_blocks", qp, qs, _typed(centroids, torch.int8, "centroids"),
+         _typed(centroid_scale, torch.float32, "centroid_scale"), bt, stride, cu, pos, block_table.shape[0], T, H, G, D,
+         page_size, N, max_kv_len, top_blocks, sink, local, dt, _typed(blocks, torch.int32, "blocks"), ptr(workspace),
+         workspace.numel(), stream_ptr(stream))
+    return blocks
+
+
+def gqa_sparse_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, blocks, scale,
+                   out=None, lse=None, workspace=None, stream=None):
+    """`gqa_decode_fp8` over the listed blocks of each row and KV head.  Returns (out, lse)."""
+    N, G, R, D = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
+    T, H, _ = q.shape
+    if blocks.dim() != 3 or blocks.shape[:2] != (T, G):
+        raise ValueError("blocks must be [T, kv_heads, top_blocks]")
+    dt = _here(q.dtype, q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, blocks, out, lse, workspace)
+    out, lse, workspace = _gqa_io(q, G, D, out, lse, workspace)
+    qp, qs = _rows(q)
+    bt, stride, cu, pos = _lanes(block_table, cu_seqlens, positions, T)
+    call("hk_gqa_sparse_fp8", qp, qs, _typed(k_cache, torch.uint8, "k_cache"), _typed(v_cache, torch.uint8, "v_cache"),
+         _typed(k_scale, torch.float32, "k_scale"), _typed(v_scale, torch.float32, "v_scale"), bt, stride, cu, pos,
+         _typed(blocks, torch.int32, "blocks"), blocks.shape[2], block_table.shape[0], T, H, G, D, R, N, scale, dt,
+         _typed(out, q.dtype, "out"), _typed(lse, torch.float32, "lse"), ptr(workspace), workspace.numel(), stream_ptr(stream))
+    return out, lse
 
 
 SAMPLING_DTYPE = np.dtype([("temperature", "<f4"), ("top_p", "<f4"), ("top_k", "<u4"),

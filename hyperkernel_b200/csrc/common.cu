@@ -121,7 +121,8 @@ int hk_check_errors(void) {
   HK_TRY_CUDA(cudaMemset(w, 0, sizeof v));
   static const char* names[] = {"?",         "pack overflow",  "pack page", "append slot",
                                 "attn page", "wait timeout",   "moe row",   "route input",
-                                "token id"};
+                                "token id",  "position",       "kv input",  "block list",
+                                "lane rows"};
   unsigned site = (unsigned)((v >> 32) & 0x7fffffff);
   unsigned detail = (unsigned)(v & 0xffffffffu);
   return hk::fail(HK_EDEVICE, "device error: %s (site %u, detail %u)",

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -33,6 +34,10 @@ enum ErrSite : unsigned {
   kErrMoeRow = 6,         // a permuted row or token index out of range
   kErrRouteInput = 7,     // non-finite router logits
   kErrToken = 8,          // a token id outside the vocabulary (the model's embedding lookup)
+  kErrPosition = 9,       // a position past the RoPE table, or past the call's max_kv_len
+  kErrKvInput = 10,       // a K or V element that is not finite, appended to the block-scaled cache
+  kErrBlockList = 11,     // a block list that is not rising or names a block past its row's position
+  kErrLaneRows = 12,      // a lane with more rows than the call's max_rows
 };
 
 }  // namespace hk
@@ -76,6 +81,37 @@ __device__ __forceinline__ float bf16_bits_to_f32(uint16_t b) {
 __device__ __forceinline__ uint16_t f32_to_bf16_bits(float f) {
   __nv_bfloat16 h = __float2bfloat16_rn(f);
   return *reinterpret_cast<uint16_t*>(&h);
+}
+
+// 8 packed bf16 or fp16 values <-> fp32.
+template <bool kF16>
+__device__ __forceinline__ void unpack8(const uint4& u, float* x) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (kF16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (kF16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <bool kF16>
+__device__ __forceinline__ uint4 pack8(const float* x) {
+  return make_uint4(pack2<kF16>(x[0], x[1]), pack2<kF16>(x[2], x[3]), pack2<kF16>(x[4], x[5]),
+                    pack2<kF16>(x[6], x[7]));
 }
 
 // e4m3 byte -> float (exact).

@@ -1,0 +1,31 @@
+// The block-scaled 8-bit GQA attention: arguments its kernels share.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace hk {
+
+struct GqaArgs {
+  const uint16_t* q;  // [T][q_heads][dim], rows q_stride elements apart
+  int64_t q_stride;
+  const uint8_t* kc;  // [num_pages][kv_heads][page_size][dim] e4m3
+  const uint8_t* vc;
+  const float* ks;    // [num_pages][kv_heads]
+  const float* vs;
+  const int32_t* bt;
+  int32_t bt_stride;
+  const int32_t* cu;
+  const int32_t* positions;
+  const int32_t* blocks;  // [T][kv_heads][top] rising block indices, -1 behind the last; null: every block
+  int32_t top;
+  int32_t num_lanes, num_tokens, q_heads, kv_heads, dim, page_size;
+  int64_t num_pages;
+  int32_t max_rows;
+  float scale;
+  uint16_t* out;  // [T][q_heads][dim]
+  float* lse;     // [T][q_heads]
+  unsigned long long* err;
+};
+
+}  // namespace hk

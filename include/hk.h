@@ -193,6 +193,119 @@ int hk_lse_merge(const float* o_parts, const float* lse_parts, int32_t n_parts, 
                  int32_t dv, uint16_t* out, float* lse_out, void* stream);
 
 /* ------------------------------------------------------------------------------------ */
+/* GQA over an 8-bit cache: QK norm with rotation, block-scaled append, attention, and    */
+/* attention over selected blocks                                                         */
+/* The reference's engine serves such layers only through its closed kernels; these take  */
+/* the same lane / block-table / position arrays as the entry points above.               */
+/* ------------------------------------------------------------------------------------ */
+
+/* Element type of the 16-bit arrays of the calls in this section (`dtype`). */
+#define HK_BF16 0
+#define HK_F16 1
+
+/* RMS norm of every query and key head with its gain, and the rotation by the row's position:
+ *   y = x / sqrt(mean(x^2) + eps) * gain, then (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)
+ * over the pairs (a, b) = (i, i + rot_dim / 2), or (2i, 2i + 1) with interleaved != 0, i <
+ * rot_dim / 2, where c and s are element i and element rot_dim / 2 + i of row positions[t] of
+ * `table` (fp32 [table_rows][rot_dim], the layout of hk_rope_table); dims past rot_dim are not
+ * rotated.  Computed in fp32, rounded once.  Row t, head h of q is at q + t * q_stride + h *
+ * head_dim (strides in elements), so q and k may be slices of a fused projection's rows; k, q_out
+ * and k_out likewise.  An output may be its own input (same address and stride), but must not overlap
+ * an input otherwise.  Gains [head_dim]; NULL = 1.  A row with a negative position is left as it
+ * is; one past table_rows is skipped and sets the device error word.  head_dim: a multiple of 8 up
+ * to 256; rot_dim: a multiple of 16, 0 = no rotation; kv_heads (or q_heads) may be 0. */
+int hk_qk_norm_rope(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                    const uint16_t* q_gain, const uint16_t* k_gain, const float* table,
+                    int64_t table_rows, int32_t rot_dim, int32_t interleaved,
+                    const int32_t* positions, int32_t num_tokens, int32_t q_heads,
+                    int32_t kv_heads, int32_t head_dim, float eps, int32_t dtype, uint16_t* q_out,
+                    int64_t q_out_stride, uint16_t* k_out, int64_t k_out_stride, void* stream);
+
+/* Appends K and V rows to the block-scaled cache: k_cache and v_cache e4m3
+ * [num_pages][kv_heads][page_size][head_dim], k_scale and v_scale fp32 [num_pages][kv_heads]; a
+ * stored q stands for q * scale of its page and head.  Rows of a lane are consecutive in the call
+ * and take consecutive slots; those in one page form a run.  For each run (from row `o` of its
+ * page), head, and K or V:
+ *   s_new = the least power of two with max|x| <= 448 * s_new (max|x| taken as at least 2^-32),
+ *   s     = s_new when o == 0, else max(s_old, s_new);  rows before o, when s > s_old, become
+ *   e4m3_rn(q * (s_old * (1/s)));  new rows are e4m3_rn_satfinite(x * (1/s)).
+ * So row 0 of a page starts its scale anew, and the scale then only grows until row 0 is written
+ * again.  Rows of the page past the run are left as they are.  A run that writes the last row of its
+ * page also writes, when `centroids` is not NULL, the page's centroid (int8
+ * [num_pages][kv_heads][head_dim], fp32 centroid_scale [num_pages][kv_heads]):
+ *   S_d = 512 * (sum over the page's rows of the stored K values),  m = max|S_d|,
+ *   centroid_d = rint(S_d * (127 / m)),  centroid_scale = k_scale * (m / (127 * 512 * page_size)).
+ * A row with a negative slot is skipped (a padding row, or one hk_pack reported).  A slot past
+ * the pool, or a row of the run's page that does not take the slot after the row before it (the
+ * same slot twice, a gap), is skipped and sets the device error word.  A value that is not
+ * finite sets the error word, does not count in max|x|, and is stored as +-448 (infinities) or 0
+ * (NaN), so a page never holds a NaN code.  Two runs in one call on the same page are a caller's
+ * error: they write it at the same time, and its rows and scale are then unspecified.
+ * head_dim 64, 128 or 256; page_size a multiple of 16 up to 256; strides in elements. */
+int hk_gqa_append_fp8(const uint16_t* k_new, int64_t k_stride, const uint16_t* v_new,
+                      int64_t v_stride, int32_t dtype, const int32_t* slot_mapping,
+                      int32_t num_tokens, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                      int64_t num_pages, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
+                      float* v_scale, int8_t* centroids, float* centroid_scale, void* stream);
+
+/* Attention over the block-scaled cache (any positive finite scales, not only powers of two):
+ * query row t of lane b sits at positions[t] and attends rows 0..positions[t] of the lane.
+ * q[T][q_heads][head_dim] (rows q_stride elements apart), out[T][q_heads][head_dim] of the same
+ * type, lse[T][q_heads] (natural log, of scale * q.k); q_heads a multiple of kv_heads, query head
+ * h reads KV head h / (q_heads / kv_heads).  Rows at and past cu_seqlens[num_lanes] are left as
+ * they are; a row with a negative position gets out 0 and lse -inf.  Positions of a lane rise by
+ * one.  max_rows and max_kv_len bound a lane's rows and KV rows (they choose the kernel and the
+ * grid); a lane past max_rows is skipped and sets the device error word, as a page that is
+ * 0 or past the pool does (its rows are not attended).  Cache rows past a lane's last position may
+ * hold anything.  A NaN code in an attended V row reaches every row of that lane in this call.
+ * workspace: hk_gqa_fp8_workspace_size bytes, 256-byte aligned. */
+size_t hk_gqa_fp8_workspace_size(int32_t num_tokens, int32_t q_heads, int32_t kv_heads,
+                                 int32_t head_dim);
+int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache,
+                      const uint8_t* v_cache, const float* k_scale, const float* v_scale,
+                      const int32_t* block_table, int32_t bt_stride, const int32_t* cu_seqlens,
+                      const int32_t* positions, int32_t num_lanes, int32_t num_tokens,
+                      int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                      int64_t num_pages, int32_t max_rows, int32_t max_kv_len, float scale,
+                      int32_t dtype, uint16_t* out, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* The blocks (pages of a lane, counted from its first) that each row and KV head reads:
+ * blocks[T][kv_heads][top_blocks] i32, rising, -1 behind the last.  With n = positions[t] /
+ * page_size + 1 blocks in sight: all of them when n <= top_blocks, else the first `sink`, the last
+ * `local` (>= 1) and the highest scores among the others, equal scores to the lower block:
+ *   u_d = sum of q over the KV head's query heads (rounded once to fp32),
+ *   c_d = rint(u_d * (127 / max|u|)),
+ *   score = fp32(sum_d c_d * centroid_d) * centroid_scale  (whole-number dot product)
+ * so the lists do not depend on the batch.  A row whose u is not finite scores 0 everywhere.
+ * Centroids are those of hk_gqa_append_fp8: every block but a row's last must be full.  Rows past
+ * cu_seqlens[num_lanes] are left as they are; one past max_kv_len gets an empty list and sets the
+ * device error word.  workspace: hk_gqa_select_workspace_size bytes, 16-byte aligned. */
+size_t hk_gqa_select_workspace_size(int32_t num_tokens, int32_t kv_heads, int32_t page_size,
+                                    int32_t max_kv_len);
+int hk_gqa_select_blocks(const uint16_t* q, int64_t q_stride, const int8_t* centroids,
+                         const float* centroid_scale, const int32_t* block_table,
+                         int32_t bt_stride, const int32_t* cu_seqlens, const int32_t* positions,
+                         int32_t num_lanes, int32_t num_tokens, int32_t q_heads, int32_t kv_heads,
+                         int32_t head_dim, int32_t page_size, int64_t num_pages,
+                         int32_t max_kv_len, int32_t top_blocks, int32_t sink, int32_t local,
+                         int32_t dtype, int32_t* blocks, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* hk_gqa_decode_fp8 restricted, for each row and KV head, to the listed blocks (rising block
+ * indices, the first -1 ends a list; hk_gqa_select_blocks writes them).  An index that does not rise,
+ * or lies past the row's position, is skipped and sets the device error word.  An empty list gives
+ * out 0 and lse -inf. */
+int hk_gqa_sparse_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache,
+                      const uint8_t* v_cache, const float* k_scale, const float* v_scale,
+                      const int32_t* block_table, int32_t bt_stride, const int32_t* cu_seqlens,
+                      const int32_t* positions, const int32_t* blocks, int32_t top_blocks,
+                      int32_t num_lanes, int32_t num_tokens, int32_t q_heads, int32_t kv_heads,
+                      int32_t head_dim, int32_t page_size, int64_t num_pages, float scale,
+                      int32_t dtype, uint16_t* out, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------ */
 /* a11  FP8 block-scaled linear                                                          */
 /* ------------------------------------------------------------------------------------ */
 
