@@ -4,7 +4,27 @@
 //
 // over the tokens j <= position of the row (and, sparse, of the row's blocks).
 //
-// One warp per (row, query head): lanes split the head's dims, online softmax in fp32.
+// Bound: HBM, the cache read once (2 * dim bytes a token and KV head).  The query rows that share a KV
+// head (rows of the lane x heads of the group) are the narrow side of the products, so the
+// tokens take the M side of mma.m16n8k16 and 8 x NT query rows the N side:
+//   S^T = K Q^T,  O^T += V^T P^T.
+// e4m3 is exact in fp16, and so is q once each row is scaled by a power of two, so the products are
+// those of the stored values; P is rounded to fp16 (2^-11, finer than the output's type).
+//
+// K and V go from global memory straight to registers: the order of k inside a product, and of the
+// dims among the M tiles of the second one, is free, so each thread's fragment is 16 consecutive
+// bytes of a token (8 at dim 64).  For V the bytes of two tokens are interleaved by prmt before the
+// conversion, which makes the transposed fragment without shared memory.  P^T reaches the layout
+// of a B fragment by movmatrix.
+//
+// With vs folded into the exponent, w_j = 2^(s_j + log2 vs - M), one running maximum M serves pages of
+// any scale, and sum_j w_j / vs is the softmax's denominator.  M is raised (and O rescaled) only when a
+// value passes it by more than 2^8, which fp16 weights have room for.
+//
+// Work split: the 16-token chunks of all (lane, KV head, row tile) problems lie end to end in
+// units of kWarps chunks, and every CTA takes an equal contiguous range of units.  Problems cut by
+// a range's end leave fp32 partials, two at most for each CTA, which gqa_merge_kernel joins in
+// the order of the ranges: results do not depend on timing.
 #include "common.cuh"
 #include "gqa_fp8.cuh"
 
@@ -12,78 +32,541 @@ namespace {
 
 using hk::GqaArgs;
 
-__device__ __forceinline__ int lane_of_row(const int32_t* __restrict__ cu, int num_lanes, int t) {
-  int lo = 0, hi = num_lanes;  // largest b with cu[b] <= t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kUnit = kWarps * 16;  // tokens
+constexpr int kMaxCtasPerSm = 2;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// What CTA i leaves for the merge: the problem its last range starts and does not finish, and whether the
+// problem it continues from the CTA before ends in it.
+struct Rec {
+  int32_t item, sub;   // problem of the open last segment (item < 0: none)
+  int32_t ends;        // the first segment was continued from the CTA before, and ends here
+  int32_t empty;       // it had no units
+};
+
+struct SplitArgs {
+  GqaArgs a;
+  int32_t is_f16;
+  int32_t group, tiles_max;
+  int32_t items;  // lanes (dense) or rows (sparse)
+  Rec* rec;       // [grid]
+  float* part;    // [grid][2][R * D + 2 R]
+};
+
+struct Item {
+  int rows, t0, len;  // query rows (tokens), first row, KV tokens (sparse: of the list)
+  int pos;            // sparse: the row's position
+  int tiles;
+  int64_t nu;         // units of one (row tile, head)
+};
+
+template <int R, bool kSparse>
+__device__ __forceinline__ Item item_of(const SplitArgs& s, int i, bool report) {
+  const GqaArgs& a = s.a;
+  Item x;
+  if (kSparse) {
+    const int total = min(a.cu[a.num_lanes], a.num_tokens);
+    x.t0 = i;
+    x.rows = i < total ? 1 : 0;
+    x.pos = x.rows ? a.positions[i] : -1;
+    x.len = x.pos < 0 ? 0 : min(a.top, x.pos / a.page_size + 1) * a.page_size;
+  } else {
+    x.t0 = a.cu[i];
+    const int t1 = min(a.cu[i + 1], a.num_tokens);
+    x.rows = x.t0 >= 0 ? max(0, t1 - x.t0) : 0;
+    if (x.rows > a.max_rows) {
+      if (report) hk_flag(a.err, hk::kErrLaneRows, (unsigned)i);
+      x.rows = 0;
+    }
+    x.pos = 0;
+    x.len = x.rows ? max(0, a.positions[t1 - 1] + 1) : 0;
   }
-  return lo;
+  x.tiles = (x.rows * s.group + R - 1) / R;
+  x.nu = max(1, (x.len + kUnit - 1) / kUnit);
+  return x;
 }
 
-template <bool kF16, int D>
-__global__ void __launch_bounds__(128) gqa_fp8_warp_kernel(GqaArgs a) {
-  constexpr int P = D / 32;
-  const int t = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (h >= a.q_heads || t >= a.cu[a.num_lanes]) return;  // rows behind the last lane stay as they are
-  const int g = h / (a.q_heads / a.kv_heads);
-  const int b = lane_of_row(a.cu, a.num_lanes, t);
-  if (a.cu[b + 1] - a.cu[b] > a.max_rows) {
-    if (lane == 0) hk_flag(a.err, hk::kErrLaneRows, (unsigned)b);
-    return;
-  }
-  const int pos = a.positions[t];
-  float q[P], acc[P];
+__device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {  // the low two bytes
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
+}
+__device__ __forceinline__ uint2 ld_once8(const void* p) {
+  uint2 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
+  return u;
+}
+
+// 16 tokens of K and V as this thread's fragments hold them.
+template <int D>
+struct Chunk {
+  uint32_t k[2][D / 16];  // tokens r, r + 8; word 4 i + m: dims 64 i + 16 c + 4 m ..
+  uint32_t v[4][D / 32];  // tokens 2c, 2c + 1, 2c + 8, 2c + 9; dims v_dim(w) ..
+};
+
+template <int D>
+__device__ __forceinline__ int v_dim(int r, int w) {
+  return D == 64 ? r * 8 + 4 * w : (w >> 2) * 128 + r * 16 + (w & 3) * 4;
+}
+
+template <int D>
+__device__ __forceinline__ void load_chunk(Chunk<D>& x, const uint8_t* k, const uint8_t* v, int r, int c) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const uint16_t w = a.q[t * a.q_stride + (int64_t)h * D + lane * P + i];
-    q[i] = kF16 ? __half2float(*reinterpret_cast<const __half*>(&w)) : bf16_bits_to_f32(w);
-    acc[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const int visible = pos < 0 ? 0 : pos / a.page_size + 1;
-  const int n = a.blocks != nullptr ? a.top : visible;
-  const int32_t* list = a.blocks != nullptr ? a.blocks + ((int64_t)t * a.kv_heads + g) * a.top : nullptr;
-  int last = -1;
-  for (int i = 0; i < n; ++i) {
-    const int blk = list != nullptr ? list[i] : i;
-    if (list != nullptr) {
-      if (blk == -1) break;
-      if (blk <= last || blk >= visible) {
-        if (lane == 0) hk_flag(a.err, hk::kErrBlockList, (unsigned)t);
-        continue;
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const uint4 u = ld_once(k + (r + 8 * h) * D + i * 64 + c * 16);
+      x.k[h][4 * i] = u.x, x.k[h][4 * i + 1] = u.y, x.k[h][4 * i + 2] = u.z, x.k[h][4 * i + 3] = u.w;
+    }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint8_t* p = v + (2 * c + (j & 1) + 8 * (j >> 1)) * D;
+    if (D == 64) {
+      const uint2 u = ld_once8(p + r * 8);
+      x.v[j][0] = u.x, x.v[j][1] = u.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 128; ++i) {
+        const uint4 u = ld_once(p + i * 128 + r * 16);
+        x.v[j][4 * i] = u.x, x.v[j][4 * i + 1] = u.y, x.v[j][4 * i + 2] = u.z, x.v[j][4 * i + 3] = u.w;
       }
-      last = blk;
-    }
-    const int page = blk < a.bt_stride ? a.bt[(int64_t)b * a.bt_stride + blk] : -1;
-    if (page <= 0 || page >= a.num_pages) {
-      if (lane == 0) hk_flag(a.err, hk::kErrAttnPage, (unsigned)b);
-      continue;
-    }
-    const int64_t base = ((int64_t)page * a.kv_heads + g) * a.page_size * D;
-    const float ks = a.ks[(int64_t)page * a.kv_heads + g] * a.scale, vs = a.vs[(int64_t)page * a.kv_heads + g];
-    const int rows = min(a.page_size, pos + 1 - blk * a.page_size);
-    for (int r = 0; r < rows; ++r) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < P; ++e) s = fmaf(q[e], e4m3_to_f32(a.kc[base + r * D + lane * P + e]), s);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      s *= ks;
-      const float m_new = fmaxf(m, s);
-      const float corr = m_new == -INFINITY ? 1.f : expf(m - m_new);
-      const float p = s == -INFINITY ? 0.f : expf(s - m_new);
-      l = l * corr + p;
-#pragma unroll
-      for (int e = 0; e < P; ++e) acc[e] = fmaf(p * vs, e4m3_to_f32(a.vc[base + r * D + lane * P + e]), acc[e] * corr);
-      m = m_new;
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that is not finite stays NaN
+}
+
+// A warp's running state: 8 NT query rows (columns 2c, 2c + 1 of each N tile in this thread).
+template <int D, int NT>
+struct State {
+  float o[D / 16][NT][4];
+  float m[NT][2], l[NT][2];
+};
+
+// One chunk into the state.  kf: ks * scale * log2 e; lsv, isv: log2 and inverse of vs; `edge`: some token is
+// past a row's position (token p0 + i is masked for a row at pos < p0 + i, and its V is not used past `len`).
+template <int D, int NT>
+__device__ __forceinline__ void step(State<D, NT>& st, Chunk<D>& x, const uint2* q_s, const float (&rowf)[NT][2],
+                                     float kf, float lsv, float isv, bool edge, int p0, int len, const int* pos_s,
+                                     int lane) {
+  const int r = lane >> 2, c = lane & 3;
+  float s[NT][4];
 #pragma unroll
-  for (int i = 0; i < P; i += 2)
-    *reinterpret_cast<uint32_t*>(a.out + ((int64_t)t * a.q_heads + h) * D + lane * P + i) = pack2<kF16>(acc[i] * inv, acc[i + 1] * inv);
-  if (lane == 0) a.lse[(int64_t)t * a.q_heads + h] = l == 0.f ? -INFINITY : m + logf(l);
+  for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const uint32_t a0 = e4m3x2_to_f16x2(x.k[0][i]), a2 = e4m3x2_to_f16x2(x.k[0][i] >> 16);
+    const uint32_t a1 = e4m3x2_to_f16x2(x.k[1][i]), a3 = e4m3x2_to_f16x2(x.k[1][i] >> 16);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint2 b = q_s[(n * (D / 16) + i) * 32 + lane];
+      mma_f16(s[n], a0, a1, a2, a3, b.x, b.y);
+    }
+  }
+  bool over = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e] * rowf[n][e & 1], kf, lsv);
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (p0 + r + 8 * (e >> 1) > pos_s[n * 8 + 2 * c + (e & 1)]) s[n][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) over |= fmaxf(s[n][e], s[n][e + 2]) > st.m[n][e] + 8.f;
+  }
+  if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float t = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+        const float m = fmaxf(st.m[n][e], t);
+        const float f = m == -INFINITY ? 1.f : exp2_approx(st.m[n][e] - m);
+        st.m[n][e] = m;
+        st.l[n][e] *= f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) st.o[j][n][e] *= f, st.o[j][n][e + 2] *= f;
+      }
+  }
+  uint32_t b0[NT], b1[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float p[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float m = st.m[n][e & 1];
+      p[e] = exp2_approx(s[n][e] - (m == -INFINITY ? 0.f : m));
+    }
+    st.l[n][0] = fmaf(p[0] + p[2], isv, st.l[n][0]);
+    st.l[n][1] = fmaf(p[1] + p[3], isv, st.l[n][1]);
+    b0[n] = transpose8x8(pack2<true>(p[0], p[1]));
+    b1[n] = transpose8x8(pack2<true>(p[2], p[3]));
+  }
+  if (edge) {  // tokens past the lane's end may hold anything, NaN codes among it
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (p0 + 2 * c + (j & 1) + 8 * (j >> 1) >= len) {
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) x.v[j][w] = 0;
+      }
+  }
+#pragma unroll
+  for (int w = 0; w < D / 32; ++w) {
+    const uint32_t lo0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140), hi0 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
+    const uint32_t lo1 = __byte_perm(x.v[2][w], x.v[3][w], 0x5140), hi1 = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
+    const uint32_t a[2][4] = {
+        {e4m3x2_to_f16x2(lo0), e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(lo1), e4m3x2_to_f16x2(lo1 >> 16)},
+        {e4m3x2_to_f16x2(hi0), e4m3x2_to_f16x2(hi0 >> 16), e4m3x2_to_f16x2(hi1), e4m3x2_to_f16x2(hi1 >> 16)}};
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_f16(st.o[2 * w + y][n], a[y][0], a[y][1], a[y][2], a[y][3], b0[n], b1[n]);
+  }
+}
+
+// Block-wide exclusive scan of one 64-bit value per thread.
+__device__ __forceinline__ int64_t block_excl_scan(int64_t v, int64_t* sums, int64_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[w];
+    all += sums[w];
+  }
+  *total = all;
+  return before + x - v;
+}
+
+template <int D, int NT>
+constexpr int split_smem() {
+  return 4 * NT * (D / 16) * 32 * 16 /* O of four warps */;
+}
+
+template <int D, int NT, bool kSparse>
+__global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) gqa_split_kernel(SplitArgs s) {
+  constexpr int R = 8 * NT;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  float4* o_s = reinterpret_cast<float4*>(dyn);  // [4][NT * D / 16][32]
+  __shared__ __align__(16) uint2 q_s[NT * (D / 16) * 32];
+  __shared__ float rowf_s[R], m_s[kWarps][R], l_s[kWarps][R];
+  __shared__ int pos_s[R];
+  __shared__ int64_t scan_s[kWarps];
+  __shared__ int64_t at_s;
+  __shared__ int item_s;
+  const GqaArgs& a = s.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
+  const int G = a.kv_heads, group = s.group;
+
+  // This CTA's range of units, and the item it begins in.
+  int64_t total = 0;
+  for (int base = 0; base < s.items; base += kThreads) {
+    const int i = base + tid;
+    int64_t n = 0, all;
+    if (i < s.items) {
+      const Item x = item_of<R, kSparse>(s, i, blockIdx.x == 0);
+      n = x.nu * x.tiles * G;
+    }
+    block_excl_scan(n, scan_s, &all);
+    total += all;
+  }
+  const int64_t u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+  Rec rec = {-1, 0, 0, u0 >= u1};
+  if (u0 < u1) {
+    int64_t carry = 0;
+    for (int base = 0; base < s.items; base += kThreads) {
+      const int i = base + tid;
+      int64_t n = 0, all;
+      if (i < s.items) {
+        const Item x = item_of<R, kSparse>(s, i, false);
+        n = x.nu * x.tiles * G;
+      }
+      const int64_t before = carry + block_excl_scan(n, scan_s, &all);
+      if (before <= u0 && u0 < before + n) item_s = i, at_s = before;
+      carry += all;
+      if (carry > u0) break;
+    }
+    __syncthreads();
+    int i = item_s;
+    int64_t begin = at_s;  // unit at which item i begins
+    Item x = item_of<R, kSparse>(s, i, false);
+    for (int64_t u = u0; u < u1;) {
+      while (u >= begin + x.nu * x.tiles * G) {
+        begin += x.nu * x.tiles * G;
+        x = item_of<R, kSparse>(s, ++i, false);
+      }
+      const int sub = (int)((u - begin) / x.nu);
+      const int first = (int)(u - begin - sub * x.nu);
+      const int last = (int)min(x.nu, first + (u1 - u));
+      const int g = sub / x.tiles, row0 = sub % x.tiles * R;
+      const int tok0 = first * kUnit, tok1 = min(x.len, last * kUnit);
+      const int lane_b = kSparse ? hk::lane_of_row(a.cu, a.num_lanes, x.t0) : i;
+      __syncthreads();
+      // Query rows: scaled by a power of two so that fp16 holds them exactly, in the order of the fragments.
+      for (int n = warp; n < R; n += kWarps) {
+        const int row = row0 + n;
+        const bool on = row < x.rows * group;
+        const int t = x.t0 + (on ? row / group : 0), h = g * group + row % group;
+        float f[D / 32];
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          f[e] = 0.f;
+          if (on) {
+            const uint16_t w = a.q[t * a.q_stride + (int64_t)h * D + lane * (D / 32) + e];
+            f[e] = s.is_f16 ? __half2float(*reinterpret_cast<const __half*>(&w)) : bf16_bits_to_f32(w);
+          }
+          top = fmaxf(top, fabsf(f[e]));
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const int ex = (int)((__float_as_uint(top) >> 23) & 255);  // 0: zero or subnormal, 255: not finite
+        const int up = ex == 255 ? 0 : min(134 - ex, 120);
+        const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const int d = lane * (D / 32) + e;
+          const int k = (d / 64) * 4 + (d % 16) / 4, cc = (d % 64) / 16;
+          reinterpret_cast<__half*>(q_s + ((n >> 3) * (D / 16) + k) * 32 + (n & 7) * 4 + cc)[d & 3] = __float2half_rn(f[e] * mul);
+        }
+        if (lane == 0) {
+          rowf_s[n] = __uint_as_float((uint32_t)(127 - up) << 23);
+          pos_s[n] = on ? a.positions[t] : INT32_MAX;
+        }
+      }
+      __syncthreads();
+      float rowf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) rowf[n][0] = rowf_s[n * 8 + 2 * c], rowf[n][1] = rowf_s[n * 8 + 2 * c + 1];
+      const int pos_min = kSparse ? x.pos : pos_s[0];  // the first row's: positions rise
+      const int len = kSparse ? x.pos + 1 : x.len;
+
+      State<D, NT> st;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        st.m[n][0] = st.m[n][1] = -INFINITY;
+        st.l[n][0] = st.l[n][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) st.o[j][n][0] = st.o[j][n][1] = st.o[j][n][2] = st.o[j][n][3] = 0.f;
+      }
+
+      // This warp's chunks: tokens tok0 + 16 warp + 128 i.  Each lane looks up the page and the scales of one
+      // of the next 32.
+      const int32_t* row_bt = a.bt + (int64_t)lane_b * a.bt_stride;
+      const int32_t* list = kSparse ? a.blocks + ((int64_t)x.t0 * G + g) * a.top : nullptr;
+      const int nchunk = tok1 > tok0 + 16 * warp ? (tok1 - tok0 - 16 * warp + kUnit - 1) / kUnit : 0;
+      for (int base = 0; base < nchunk; base += 32) {
+        int64_t offset = -1;  // of the chunk in the cache; -1: not to be read
+        int p0 = 0;           // its first token, in the lane
+        float kf = 0.f, vs = 1.f;
+        if (base + lane < nchunk) {
+          const int j = tok0 + 16 * warp + kUnit * (base + lane);
+          const int idx = j / a.page_size;
+          int blk = idx;
+          const int r16 = j - idx * a.page_size;
+          if (kSparse) {
+            blk = list[idx];
+            const int before = idx > 0 ? list[idx - 1] : -1;
+            if (blk != -1 && (blk <= before || (idx > 0 && before < 0) || blk > x.pos / a.page_size)) {
+              hk_flag(a.err, hk::kErrBlockList, (unsigned)x.t0);
+              blk = -1;
+            }
+          }
+          if (blk >= 0) {
+            p0 = blk * a.page_size + r16;
+            const int page = blk < a.bt_stride ? row_bt[blk] : -1;
+            if (page <= 0 || page >= a.num_pages) {
+              hk_flag(a.err, hk::kErrAttnPage, (unsigned)lane_b);
+            } else {
+              offset = (((int64_t)page * G + g) * a.page_size + r16) * D;
+              kf = a.ks[(int64_t)page * G + g] * (a.scale * kLog2e);
+              vs = fmaxf(a.vs[(int64_t)page * G + g], 7.8886090522101181e-31f);
+            }
+          }
+        }
+        const float lsv = log2f(vs), isv = 1.f / vs;
+        const int m = min(32, nchunk - base);
+        Chunk<D> buf[2];
+        int64_t off = __shfl_sync(0xffffffffu, offset, 0);
+        if (off >= 0) load_chunk<D>(buf[0], a.kc + off, a.vc + off, r, c);
+#pragma unroll 1
+        for (int e = 0; e < m; e += 2) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            if (e + y >= m) break;
+            const int64_t next = __shfl_sync(0xffffffffu, offset, min(e + y + 1, 31));
+            if (next >= 0 && e + y + 1 < m) load_chunk<D>(buf[y ^ 1], a.kc + next, a.vc + next, r, c);
+            const int p = __shfl_sync(0xffffffffu, p0, e + y);
+            const float fk = __shfl_sync(0xffffffffu, kf, e + y), fl = __shfl_sync(0xffffffffu, lsv, e + y),
+                        fi = __shfl_sync(0xffffffffu, isv, e + y);
+            if (off >= 0) step<D, NT>(st, buf[y], q_s, rowf, fk, fl, fi, p + 15 > pos_min, p, len, pos_s, lane);
+            off = next;
+          }
+        }
+      }
+
+      // Join the warps: maxima through shared memory, then O pairwise (4 + 4, 2 + 2, 1 + 1).
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float l = st.l[n][e];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+          if (r == 0) m_s[warp][n * 8 + 2 * c + e] = st.m[n][e], l_s[warp][n * 8 + 2 * c + e] = l;
+        }
+      __syncthreads();
+      float top[NT][2], sum[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = n * 8 + 2 * c + e;
+          float m = -INFINITY, l = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) m = fmaxf(m, m_s[w][row]);
+          const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) l += l_s[w][row] * exp2_approx(m_s[w][row] - mm);
+          top[n][e] = m, sum[n][e] = l;
+          const float f = exp2_approx(st.m[n][e] - mm);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) st.o[j][n][e] *= f, st.o[j][n][e + 2] *= f;
+        }
+#pragma unroll
+      for (int half = kWarps / 2; half > 0; half >>= 1) {
+        if (warp >= half && warp < 2 * half) {
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              o_s[(((warp - half) * (D / 16) + j) * NT + n) * 32 + lane] = make_float4(st.o[j][n][0], st.o[j][n][1], st.o[j][n][2], st.o[j][n][3]);
+        }
+        __syncthreads();
+        if (warp < half) {
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float4 y = o_s[((warp * (D / 16) + j) * NT + n) * 32 + lane];
+              st.o[j][n][0] += y.x, st.o[j][n][1] += y.y, st.o[j][n][2] += y.z, st.o[j][n][3] += y.w;
+            }
+        }
+        __syncthreads();
+      }
+      const bool starts = first == 0, ends = last == x.nu;
+      if (warp == 0) {
+        float* part = s.part + ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (R * D + 2 * R);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = n * 8 + 2 * c + e, at = row0 + row;
+            if (starts && ends) {
+              if (at >= x.rows * group) continue;
+              const int64_t y = (int64_t)(x.t0 + at / group) * a.q_heads + g * group + at % group;
+              const float inv = sum[n][e] == 0.f ? 0.f : 1.f / sum[n][e];
+#pragma unroll
+              for (int w = 0; w < D / 32; ++w) {
+                const float o0 = st.o[2 * w][n][e] * inv, o1 = st.o[2 * w][n][e + 2] * inv, o2 = st.o[2 * w + 1][n][e] * inv,
+                            o3 = st.o[2 * w + 1][n][e + 2] * inv;
+                uint2 u;
+                if (s.is_f16) u = make_uint2(pack2<true>(o0, o1), pack2<true>(o2, o3));
+                else u = make_uint2(pack2<false>(o0, o1), pack2<false>(o2, o3));
+                *reinterpret_cast<uint2*>(a.out + y * D + v_dim<D>(r, w)) = u;
+              }
+              if (r == 0) a.lse[y] = sum[n][e] == 0.f ? -INFINITY : fmaf(top[n][e], kLn2, logf(sum[n][e]));
+            } else {
+#pragma unroll
+              for (int w = 0; w < D / 32; ++w)
+                *reinterpret_cast<float4*>(part + row * D + v_dim<D>(r, w)) =
+                    make_float4(st.o[2 * w][n][e], st.o[2 * w][n][e + 2], st.o[2 * w + 1][n][e], st.o[2 * w + 1][n][e + 2]);
+              if (r == 0) part[R * D + row] = top[n][e], part[R * D + R + row] = sum[n][e];
+            }
+          }
+      }
+      if (starts && !ends) rec.item = i, rec.sub = sub;
+      if (!starts && ends) rec.ends = 1;
+      u += last - first;
+    }
+  }
+  if (tid == 0) s.rec[blockIdx.x] = rec;
+}
+
+// Joins the partials of the problem that CTA blockIdx.x of the split kernel began and left open; blockIdx.y
+// picks 8 of its rows.  Warp w holds row w, lanes its dims.
+template <int D, int NT, bool kSparse>
+__global__ void __launch_bounds__(256) gqa_merge_kernel(SplitArgs s, int ctas) {
+  constexpr int R = 8 * NT, P = D / 32;
+  const GqaArgs& a = s.a;
+  const Rec rec = s.rec[blockIdx.x];
+  if (rec.item < 0) return;
+  const Item x = item_of<R, kSparse>(s, rec.item, false);
+  const int g = rec.sub / x.tiles, row0 = rec.sub % x.tiles * R;
+  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), at = row0 + row;
+  if (at >= x.rows * s.group) return;
+  constexpr int64_t kPart = R * D + 2 * R;
+  const float* part = s.part + ((int64_t)blockIdx.x * 2 + 1) * kPart;
+  float m = part[R * D + row], l = part[R * D + R + row], o[P];
+#pragma unroll
+  for (int e = 0; e < P; ++e) o[e] = part[row * D + lane * P + e];
+  for (int i = blockIdx.x + 1; i < ctas; ++i) {
+    if (s.rec[i].empty) continue;
+    part = s.part + (int64_t)i * 2 * kPart;
+    const float pm = part[R * D + row], pl = part[R * D + R + row];
+    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
+    const float f = exp2_approx(m - ref), pf = exp2_approx(pm - ref);
+    m = top;
+    l = l * f + pl * pf;
+#pragma unroll
+    for (int e = 0; e < P; ++e) o[e] = o[e] * f + part[row * D + lane * P + e] * pf;
+    if (s.rec[i].ends) break;
+  }
+  const int64_t y = (int64_t)(x.t0 + at / s.group) * a.q_heads + g * s.group + at % s.group;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < P; e += 2) {
+    const float lo = o[e] * inv, hi = o[e + 1] * inv;
+    *reinterpret_cast<uint32_t*>(a.out + y * D + lane * P + e) = s.is_f16 ? pack2<true>(lo, hi) : pack2<false>(lo, hi);
+  }
+  if (lane == 0) a.lse[y] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
 }
 
 int check(const char* name, const GqaArgs& a, int32_t dtype) {
@@ -102,22 +585,59 @@ int check(const char* name, const GqaArgs& a, int32_t dtype) {
   return HK_OK;
 }
 
-int launch(GqaArgs& a, int32_t dtype, cudaStream_t s) {
-  a.err = hk::err_word();
-  const dim3 grid(a.num_tokens, (a.q_heads + 3) / 4);
-#define HK_GQA(D)                                                            \
-  case D:                                                                    \
-    if (dtype == HK_F16) gqa_fp8_warp_kernel<true, D><<<grid, 128, 0, s>>>(a); \
-    else gqa_fp8_warp_kernel<false, D><<<grid, 128, 0, s>>>(a);              \
-    break
-  switch (a.dim) {
-    HK_GQA(64);
-    HK_GQA(128);
-    HK_GQA(256);
+// N tiles for `rows` query rows of a problem: 1 to 4, at most 2 at dim 256 (registers).
+int n_tiles(int64_t rows, int dim) {
+  const int64_t n = (rows + 7) / 8, most = dim == 256 ? 2 : 4;
+  return (int)(n < most ? n : most);
+}
+
+size_t part_floats(int nt, int dim) { return (size_t)8 * nt * dim + 16 * nt; }
+
+template <int D, int NT, bool kSparse>
+int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
+  constexpr int smem = split_smem<D, NT>();
+  static_assert(smem <= 128 * 1024, "O of four warps");
+  const int most = hk::sm_count() * (NT == 1 && D <= 128 ? 2 : 1);
+  const int grid = (int)(units < most ? units : most);
+  if (smem > 32 * 1024)  // set on every call: cheap, and right on every device
+    HK_TRY_CUDA(cudaFuncSetAttribute(gqa_split_kernel<D, NT, kSparse>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  gqa_split_kernel<D, NT, kSparse><<<grid, kThreads, smem, stream>>>(s);
+  HK_TRY_LAUNCH("gqa_split_kernel");
+  if (grid > 1) {
+    gqa_merge_kernel<D, NT, kSparse><<<dim3(grid, NT), 256, 0, stream>>>(s, grid);
+    HK_TRY_LAUNCH("gqa_merge_kernel");
   }
-#undef HK_GQA
-  HK_TRY_LAUNCH("gqa_fp8_warp_kernel");
   return HK_OK;
+}
+
+template <bool kSparse>
+int launch(const GqaArgs& a, int32_t dtype, int64_t rows, int64_t units, void* workspace, cudaStream_t stream) {
+  SplitArgs s;
+  s.a = a;
+  s.a.err = hk::err_word();
+  s.is_f16 = dtype == HK_F16;
+  s.group = a.q_heads / a.kv_heads;
+  s.items = kSparse ? a.num_tokens : a.num_lanes;
+  s.rec = (Rec*)workspace;
+  s.part = (float*)((uint8_t*)workspace + (size_t)hk::sm_count() * kMaxCtasPerSm * sizeof(Rec));
+  const int nt = n_tiles(rows * s.group, a.dim);
+  switch (a.dim * 8 + nt) {
+#define HK_GQA(D, NT) \
+  case D * 8 + NT:    \
+    return launch_one<D, NT, kSparse>(s, units, stream)
+    HK_GQA(64, 1);
+    HK_GQA(64, 2);
+    HK_GQA(64, 3);
+    HK_GQA(64, 4);
+    HK_GQA(128, 1);
+    HK_GQA(128, 2);
+    HK_GQA(128, 3);
+    HK_GQA(128, 4);
+    HK_GQA(256, 1);
+    HK_GQA(256, 2);
+#undef HK_GQA
+  }
+  return hk::fail(HK_EINVAL, "no kernel for dim %d", a.dim);
 }
 
 }  // namespace
@@ -125,8 +645,10 @@ int launch(GqaArgs& a, int32_t dtype, cudaStream_t s) {
 extern "C" {
 
 size_t hk_gqa_fp8_workspace_size(int32_t num_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
-  (void)num_tokens, (void)q_heads, (void)kv_heads, (void)head_dim;
-  return 256;
+  if (num_tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
+  const int nt = n_tiles((int64_t)num_tokens * (q_heads / kv_heads > 0 ? q_heads / kv_heads : 1), head_dim);
+  const size_t ctas = (size_t)hk::sm_count() * kMaxCtasPerSm;
+  return (ctas * (sizeof(Rec) + 2 * part_floats(nt, head_dim) * sizeof(float)) + 255) / 256 * 256;
 }
 
 int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache, const uint8_t* v_cache,
@@ -145,7 +667,10 @@ int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cach
   if (workspace == nullptr || workspace_bytes < hk_gqa_fp8_workspace_size(num_tokens, q_heads, kv_heads, head_dim))
     return hk::fail(HK_ESPACE, "hk_gqa_decode_fp8: workspace of %zu bytes is too small", workspace_bytes);
   HK_TRY(hk::ensure_device());
-  return launch(a, dtype, (cudaStream_t)stream);
+  const int64_t rows = max_rows < num_tokens ? max_rows : num_tokens;
+  const int64_t tiles = rows * (q_heads / kv_heads) / 8 + 1;
+  const int64_t units = (int64_t)(num_lanes < num_tokens ? num_lanes : num_tokens) * kv_heads * tiles * (max_kv_len / kUnit + 1);
+  return launch<false>(a, dtype, rows > 0 ? rows : 1, units, workspace, (cudaStream_t)stream);
 }
 
 int hk_gqa_sparse_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache, const uint8_t* v_cache,
@@ -165,7 +690,9 @@ int hk_gqa_sparse_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cach
   if (workspace == nullptr || workspace_bytes < hk_gqa_fp8_workspace_size(num_tokens, q_heads, kv_heads, head_dim))
     return hk::fail(HK_ESPACE, "hk_gqa_sparse_fp8: workspace of %zu bytes is too small", workspace_bytes);
   HK_TRY(hk::ensure_device());
-  return launch(a, dtype, (cudaStream_t)stream);
+  const int group = q_heads / kv_heads;
+  const int64_t units = (int64_t)num_tokens * kv_heads * (group / 8 + 1) * ((int64_t)top_blocks * page_size / kUnit + 1);
+  return launch<true>(a, dtype, 1, units, workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -28,4 +28,14 @@ struct GqaArgs {
   unsigned long long* err;
 };
 
+// The lane of row t: the largest b with cu[b] <= t.
+__device__ __forceinline__ int lane_of_row(const int32_t* __restrict__ cu, int num_lanes, int t) {
+  int lo = 0, hi = num_lanes;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
 }  // namespace hk

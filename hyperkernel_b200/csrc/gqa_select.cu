@@ -13,6 +13,7 @@
 // scores' order, a radix select for the top_blocks-th key (8 bits a pass), and one ordered pass
 // that writes the chosen indices rising.
 #include "common.cuh"
+#include "gqa_fp8.cuh"
 
 namespace {
 
@@ -35,15 +36,6 @@ struct SelectArgs {
   uint32_t* keys;  // [T][kv_heads][max_blocks]
   unsigned long long* err;
 };
-
-__device__ __forceinline__ int lane_of_row(const int32_t* __restrict__ cu, int num_lanes, int t) {
-  int lo = 0, hi = num_lanes;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid;
-  }
-  return lo;
-}
 
 __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t b = __float_as_uint(f);
@@ -72,7 +64,7 @@ __global__ void __launch_bounds__(kThreads) gqa_select_kernel(SelectArgs a) {
     for (int i = tid; i < a.top; i += kThreads) list[i] = i < n ? i : -1;
     return;
   }
-  const int b = lane_of_row(a.cu, a.num_lanes, t);
+  const int b = hk::lane_of_row(a.cu, a.num_lanes, t);
   const int group = a.q_heads / a.kv_heads;
   float mine = 0.f;
   if (tid < a.dim) {

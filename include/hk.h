@@ -293,8 +293,9 @@ int hk_gqa_select_blocks(const uint16_t* q, int64_t q_stride, const int8_t* cent
                          void* stream);
 
 /* hk_gqa_decode_fp8 restricted, for each row and KV head, to the listed blocks (rising block
- * indices, the first -1 ends a list; hk_gqa_select_blocks writes them).  An index that does not rise,
- * or lies past the row's position, is skipped and sets the device error word.  An empty list gives
+ * indices, -1 behind the last; hk_gqa_select_blocks writes them).  An index that does not rise above
+ * the entry before it, follows a -1 or lies past the row's position is skipped and sets the device
+ * error word.  An empty list gives
  * out 0 and lse -inf. */
 int hk_gqa_sparse_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache,
                       const uint8_t* v_cache, const float* k_scale, const float* v_scale,
