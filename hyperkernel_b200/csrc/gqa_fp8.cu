@@ -32,10 +32,17 @@ namespace {
 
 using hk::GqaArgs;
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = kWarps * 16;  // tokens
-constexpr int kMaxCtasPerSm = 2;
+constexpr int kMaxCtasPerSm = 5;
+constexpr int kWaves = 4;           // ranges for each resident CTA, when there is work for them
+constexpr int kRangeUnits = 16;     // units below which a range is not worth a CTA's start
+
+// CTAs that an SM holds (by registers: 128 threads of at most 96, 128, 168 or 255).
+constexpr int ctas_per_sm(int d, int nt) {
+  return d * nt <= 64 ? 5 : d * nt <= 128 ? 4 : d * nt <= 384 ? 3 : 2;
+}
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -44,7 +51,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct Rec {
   int32_t item, sub;   // problem of the open last segment (item < 0: none)
   int32_t ends;        // the first segment was continued from the CTA before, and ends here
-  int32_t empty;       // it had no units
+  int32_t pad;
 };
 
 struct SplitArgs {
@@ -52,6 +59,7 @@ struct SplitArgs {
   int32_t is_f16;
   int32_t group, tiles_max;
   int32_t items;  // lanes (dense) or rows (sparse)
+  int32_t resident;  // CTAs that run at once
   Rec* rec;       // [grid]
   float* part;    // [grid][2][R * D + 2 R]
 };
@@ -96,9 +104,11 @@ __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {  // the low two bytes
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four e4m3 bytes as two fp16 pairs (exact).
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -124,38 +134,37 @@ __device__ __forceinline__ uint2 ld_once8(const void* p) {
   return u;
 }
 
-// 16 tokens of K and V as this thread's fragments hold them.
-template <int D>
-struct Chunk {
-  uint32_t k[2][D / 16];  // tokens r, r + 8; word 4 i + m: dims 64 i + 16 c + 4 m ..
-  uint32_t v[4][D / 32];  // tokens 2c, 2c + 1, 2c + 8, 2c + 9; dims v_dim(w) ..
-};
-
 template <int D>
 __device__ __forceinline__ int v_dim(int r, int w) {
   return D == 64 ? r * 8 + 4 * w : (w >> 2) * 128 + r * 16 + (w & 3) * 4;
 }
 
+// K of 16 tokens as this thread's fragments hold it: tokens r and r + 8; word 4 i + m: dims 64 i + 16 c + 4 m ...
 template <int D>
-__device__ __forceinline__ void load_chunk(Chunk<D>& x, const uint8_t* k, const uint8_t* v, int r, int c) {
+__device__ __forceinline__ void load_k(uint32_t (&x)[2][D / 16], const uint8_t* k, int r, int c) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       const uint4 u = ld_once(k + (r + 8 * h) * D + i * 64 + c * 16);
-      x.k[h][4 * i] = u.x, x.k[h][4 * i + 1] = u.y, x.k[h][4 * i + 2] = u.z, x.k[h][4 * i + 3] = u.w;
+      x[h][4 * i] = u.x, x[h][4 * i + 1] = u.y, x[h][4 * i + 2] = u.z, x[h][4 * i + 3] = u.w;
     }
+}
+
+// V of 16 tokens: tokens 2c, 2c + 1, 2c + 8, 2c + 9; word w: dims v_dim(r, w) ...
+template <int D>
+__device__ __forceinline__ void load_v(uint32_t (&x)[4][D / 32], const uint8_t* v, int r, int c) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint8_t* p = v + (2 * c + (j & 1) + 8 * (j >> 1)) * D;
     if (D == 64) {
       const uint2 u = ld_once8(p + r * 8);
-      x.v[j][0] = u.x, x.v[j][1] = u.y;
+      x[j][0] = u.x, x[j][1] = u.y;
     } else {
 #pragma unroll
       for (int i = 0; i < D / 128; ++i) {
         const uint4 u = ld_once(p + i * 128 + r * 16);
-        x.v[j][4 * i] = u.x, x.v[j][4 * i + 1] = u.y, x.v[j][4 * i + 2] = u.z, x.v[j][4 * i + 3] = u.w;
+        x[j][4 * i] = u.x, x[j][4 * i + 1] = u.y, x[j][4 * i + 2] = u.z, x[j][4 * i + 3] = u.w;
       }
     }
   }
@@ -168,31 +177,36 @@ struct State {
   float m[NT][2], l[NT][2];
 };
 
-// One chunk into the state.  kf: ks * scale * log2 e; lsv, isv: log2 and inverse of vs; `edge`: some token is
-// past a row's position (token p0 + i is masked for a row at pos < p0 + i, and its V is not used past `len`).
+// S = K Q^T of one chunk: column n * 8 + 2c + (e & 1), token r + 8 (e >> 1).
 template <int D, int NT>
-__device__ __forceinline__ void step(State<D, NT>& st, Chunk<D>& x, const uint2* q_s, const float (&rowf)[NT][2],
-                                     float kf, float lsv, float isv, bool edge, int p0, int len, const int* pos_s,
-                                     int lane) {
-  const int r = lane >> 2, c = lane & 3;
-  float s[NT][4];
+__device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&k)[2][D / 16], const uint2* q_s, int lane) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    const uint32_t a0 = e4m3x2_to_f16x2(x.k[0][i]), a2 = e4m3x2_to_f16x2(x.k[0][i] >> 16);
-    const uint32_t a1 = e4m3x2_to_f16x2(x.k[1][i]), a3 = e4m3x2_to_f16x2(x.k[1][i] >> 16);
+    uint32_t a0, a1, a2, a3;
+    e4m3x4_to_f16x4(k[0][i], a0, a2);
+    e4m3x4_to_f16x4(k[1][i], a1, a3);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const uint2 b = q_s[(n * (D / 16) + i) * 32 + lane];
       mma_f16(s[n], a0, a1, a2, a3, b.x, b.y);
     }
   }
+}
+
+// The scores of one chunk become weights (B fragments of P) and enter the running sums.  kf: ks * scale *
+// log2 e; lsv, isv: log2 and inverse of vs; `edge`: some token is past a row's position.
+template <int D, int NT>
+__device__ __forceinline__ void weigh(State<D, NT>& st, float (&s)[NT][4], uint32_t (&b)[NT][2], const float (&rowf)[NT][2],
+                                      float kf, float lsv, float isv, bool edge, int p0, const int* pos_s, int lane) {
+  const int r = lane >> 2, c = lane & 3;
   bool over = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    const float f0 = rowf[n][0] * kf, f1 = rowf[n][1] * kf;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e] * rowf[n][e & 1], kf, lsv);
+    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], e & 1 ? f1 : f0, lsv);
     if (edge) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -217,7 +231,6 @@ __device__ __forceinline__ void step(State<D, NT>& st, Chunk<D>& x, const uint2*
         for (int j = 0; j < D / 16; ++j) st.o[j][n][e] *= f, st.o[j][n][e + 2] *= f;
       }
   }
-  uint32_t b0[NT], b1[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float p[4];
@@ -228,28 +241,26 @@ __device__ __forceinline__ void step(State<D, NT>& st, Chunk<D>& x, const uint2*
     }
     st.l[n][0] = fmaf(p[0] + p[2], isv, st.l[n][0]);
     st.l[n][1] = fmaf(p[1] + p[3], isv, st.l[n][1]);
-    b0[n] = transpose8x8(pack2<true>(p[0], p[1]));
-    b1[n] = transpose8x8(pack2<true>(p[2], p[3]));
+    b[n][0] = transpose8x8(pack2<true>(p[0], p[1]));
+    b[n][1] = transpose8x8(pack2<true>(p[2], p[3]));
   }
-  if (edge) {  // tokens past the lane's end may hold anything, NaN codes among it
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (p0 + 2 * c + (j & 1) + 8 * (j >> 1) >= len) {
-#pragma unroll
-        for (int w = 0; w < D / 32; ++w) x.v[j][w] = 0;
-      }
-  }
+}
+
+// O += V^T P of one chunk.
+template <int D, int NT>
+__device__ __forceinline__ void values(State<D, NT>& st, const uint32_t (&v)[4][D / 32], const uint32_t (&b)[NT][2]) {
 #pragma unroll
   for (int w = 0; w < D / 32; ++w) {
-    const uint32_t lo0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140), hi0 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
-    const uint32_t lo1 = __byte_perm(x.v[2][w], x.v[3][w], 0x5140), hi1 = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
-    const uint32_t a[2][4] = {
-        {e4m3x2_to_f16x2(lo0), e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(lo1), e4m3x2_to_f16x2(lo1 >> 16)},
-        {e4m3x2_to_f16x2(hi0), e4m3x2_to_f16x2(hi0 >> 16), e4m3x2_to_f16x2(hi1), e4m3x2_to_f16x2(hi1 >> 16)}};
+    uint32_t a[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      e4m3x4_to_f16x4(__byte_perm(v[2 * h][w], v[2 * h + 1][w], 0x5140), a[0][2 * h], a[0][2 * h + 1]);
+      e4m3x4_to_f16x4(__byte_perm(v[2 * h][w], v[2 * h + 1][w], 0x7362), a[1][2 * h], a[1][2 * h + 1]);
+    }
 #pragma unroll
     for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_f16(st.o[2 * w + y][n], a[y][0], a[y][1], a[y][2], a[y][3], b0[n], b1[n]);
+      for (int n = 0; n < NT; ++n) mma_f16(st.o[2 * w + y][n], a[y][0], a[y][1], a[y][2], a[y][3], b[n][0], b[n][1]);
   }
 }
 
@@ -277,14 +288,14 @@ __device__ __forceinline__ int64_t block_excl_scan(int64_t v, int64_t* sums, int
 
 template <int D, int NT>
 constexpr int split_smem() {
-  return 4 * NT * (D / 16) * 32 * 16 /* O of four warps */;
+  return kWarps / 2 * NT * (D / 16) * 32 * 16;  // O of half the warps
 }
 
 template <int D, int NT, bool kSparse>
-__global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) gqa_split_kernel(SplitArgs s) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel(SplitArgs s) {
   constexpr int R = 8 * NT;
   extern __shared__ __align__(16) uint8_t dyn[];
-  float4* o_s = reinterpret_cast<float4*>(dyn);  // [4][NT * D / 16][32]
+  float4* o_s = reinterpret_cast<float4*>(dyn);  // [kWarps / 2][NT * D / 16][32]
   __shared__ __align__(16) uint2 q_s[NT * (D / 16) * 32];
   __shared__ float rowf_s[R], m_s[kWarps][R], l_s[kWarps][R];
   __shared__ int pos_s[R];
@@ -307,8 +318,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) gqa_spl
     block_excl_scan(n, scan_s, &all);
     total += all;
   }
-  const int64_t u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
-  Rec rec = {-1, 0, 0, u0 >= u1};
+  // Several ranges for each resident CTA even out what SMs get done; short problems use all CTAs once.
+  const int64_t ranges = max(min((int64_t)gridDim.x, total / kRangeUnits), min((int64_t)s.resident, total));
+  const int64_t cta = blockIdx.x;
+  const int64_t u0 = cta < ranges ? total * cta / ranges : 0, u1 = cta < ranges ? total * (cta + 1) / ranges : 0;
+  Rec rec = {-1, 0, 0, 0};
   if (u0 < u1) {
     int64_t carry = 0;
     for (int base = 0; base < s.items; base += kThreads) {
@@ -423,22 +437,37 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) gqa_spl
         }
         const float lsv = log2f(vs), isv = 1.f / vs;
         const int m = min(32, nchunk - base);
-        Chunk<D> buf[2];
+        // K of the next chunk is asked for once this one's scores are computed, V once its product is: one
+        // chunk in registers, and the loads of the next in flight behind the rest of the step.
+        uint32_t k[2][D / 16], v[4][D / 32];
         int64_t off = __shfl_sync(0xffffffffu, offset, 0);
-        if (off >= 0) load_chunk<D>(buf[0], a.kc + off, a.vc + off, r, c);
+        if (off >= 0) load_k<D>(k, a.kc + off, r, c), load_v<D>(v, a.vc + off, r, c);
 #pragma unroll 1
-        for (int e = 0; e < m; e += 2) {
+        for (int e = 0; e < m; ++e) {
+          int64_t next = __shfl_sync(0xffffffffu, offset, min(e + 1, 31));
+          if (e + 1 >= m) next = -1;
+          const int p = __shfl_sync(0xffffffffu, p0, e);
+          const float fk = __shfl_sync(0xffffffffu, kf, e), fl = __shfl_sync(0xffffffffu, lsv, e),
+                      fi = __shfl_sync(0xffffffffu, isv, e);
+          const bool edge = p + 15 > pos_min;
+          float sc[NT][4];
+          uint32_t pb[NT][2];
+          if (off >= 0) scores<D, NT>(sc, k, q_s, lane);
+          if (next >= 0) load_k<D>(k, a.kc + next, r, c);
+          if (off >= 0) {
+            weigh<D, NT>(st, sc, pb, rowf, fk, fl, fi, edge, p, pos_s, lane);
+            if (edge) {  // tokens past the lane's end may hold anything, NaN codes among it
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            if (e + y >= m) break;
-            const int64_t next = __shfl_sync(0xffffffffu, offset, min(e + y + 1, 31));
-            if (next >= 0 && e + y + 1 < m) load_chunk<D>(buf[y ^ 1], a.kc + next, a.vc + next, r, c);
-            const int p = __shfl_sync(0xffffffffu, p0, e + y);
-            const float fk = __shfl_sync(0xffffffffu, kf, e + y), fl = __shfl_sync(0xffffffffu, lsv, e + y),
-                        fi = __shfl_sync(0xffffffffu, isv, e + y);
-            if (off >= 0) step<D, NT>(st, buf[y], q_s, rowf, fk, fl, fi, p + 15 > pos_min, p, len, pos_s, lane);
-            off = next;
+              for (int j = 0; j < 4; ++j)
+                if (p + 2 * c + (j & 1) + 8 * (j >> 1) >= len) {
+#pragma unroll
+                  for (int w = 0; w < D / 32; ++w) v[j][w] = 0;
+                }
+            }
+            values<D, NT>(st, v, pb);
           }
+          if (next >= 0) load_v<D>(v, a.vc + next, r, c);
+          off = next;
         }
       }
 
@@ -548,7 +577,6 @@ __global__ void __launch_bounds__(256) gqa_merge_kernel(SplitArgs s, int ctas) {
 #pragma unroll
   for (int e = 0; e < P; ++e) o[e] = part[row * D + lane * P + e];
   for (int i = blockIdx.x + 1; i < ctas; ++i) {
-    if (s.rec[i].empty) continue;
     part = s.part + (int64_t)i * 2 * kPart;
     const float pm = part[R * D + row], pl = part[R * D + R + row];
     const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
@@ -596,9 +624,11 @@ size_t part_floats(int nt, int dim) { return (size_t)8 * nt * dim + 16 * nt; }
 template <int D, int NT, bool kSparse>
 int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
   constexpr int smem = split_smem<D, NT>();
-  static_assert(smem <= 128 * 1024, "O of four warps");
-  const int most = hk::sm_count() * (NT == 1 && D <= 128 ? 2 : 1);
-  const int grid = (int)(units < most ? units : most);
+  s.resident = hk::sm_count() * ctas_per_sm(D, NT);
+  const int64_t wide = units / kRangeUnits < (int64_t)s.resident * kWaves ? units / kRangeUnits : (int64_t)s.resident * kWaves;
+  const int64_t once = units < s.resident ? units : s.resident;
+  const int grid = (int)(wide > once ? wide : once);
+  s.resident = (int)(s.resident < grid ? s.resident : grid);
   if (smem > 32 * 1024)  // set on every call: cheap, and right on every device
     HK_TRY_CUDA(cudaFuncSetAttribute(gqa_split_kernel<D, NT, kSparse>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   gqa_split_kernel<D, NT, kSparse><<<grid, kThreads, smem, stream>>>(s);
@@ -619,7 +649,7 @@ int launch(const GqaArgs& a, int32_t dtype, int64_t rows, int64_t units, void* w
   s.group = a.q_heads / a.kv_heads;
   s.items = kSparse ? a.num_tokens : a.num_lanes;
   s.rec = (Rec*)workspace;
-  s.part = (float*)((uint8_t*)workspace + (size_t)hk::sm_count() * kMaxCtasPerSm * sizeof(Rec));
+  s.part = (float*)((uint8_t*)workspace + (size_t)hk::sm_count() * kMaxCtasPerSm * kWaves * sizeof(Rec));
   const int nt = n_tiles(rows * s.group, a.dim);
   switch (a.dim * 8 + nt) {
 #define HK_GQA(D, NT) \
@@ -647,8 +677,12 @@ extern "C" {
 size_t hk_gqa_fp8_workspace_size(int32_t num_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (num_tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
   const int nt = n_tiles((int64_t)num_tokens * (q_heads / kv_heads > 0 ? q_heads / kv_heads : 1), head_dim);
-  const size_t ctas = (size_t)hk::sm_count() * kMaxCtasPerSm;
-  return (ctas * (sizeof(Rec) + 2 * part_floats(nt, head_dim) * sizeof(float)) + 255) / 256 * 256;
+  size_t most = 0;  // over the tile counts that a call with these sizes can pick
+  for (int n = 1; n <= nt; ++n) {
+    const size_t part = ctas_per_sm(head_dim, n) * 2 * part_floats(n, head_dim) * sizeof(float);
+    most = most > part ? most : part;
+  }
+  return (size_t)hk::sm_count() * kWaves * (kMaxCtasPerSm * sizeof(Rec) + most);
 }
 
 int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache, const uint8_t* v_cache,
