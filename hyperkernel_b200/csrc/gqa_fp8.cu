@@ -11,11 +11,14 @@
 // e4m3 is exact in fp16, and so is q once each row is scaled by a power of two, so the products are
 // those of the stored values; P is rounded to fp16 (2^-11, finer than the output's type).
 //
-// K and V go from global memory straight to registers: the order of k inside a product, and of the
-// dims among the M tiles of the second one, is free, so each thread's fragment is 16 consecutive
-// bytes of a token (8 at dim 64).  For V the bytes of two tokens are interleaved by prmt before the
-// conversion, which makes the transposed fragment without shared memory.  P^T reaches the layout
-// of a B fragment by movmatrix.
+// Every warp streams 16-token chunks through a ring of its own in shared memory, filled by TMA (a chunk
+// of one page and head is contiguous: 16 * dim bytes), so bytes in flight cost no registers and
+// no barrier joins warps.  The order of k inside a product, and of the dims among the M tiles of
+// the second one, is free, so each thread's fragments are runs of 16 bytes of a token (8 for V at
+// dim 64), and TMA's 128-byte swizzle keeps those reads free of bank conflicts (2-way at most
+// for V at dims 64 and 256).  For V the bytes of two tokens are interleaved by prmt before the
+// conversion, which makes the transposed fragment.  P^T reaches the layout of a B fragment by
+// movmatrix.
 //
 // With vs folded into the exponent, w_j = 2^(s_j + log2 vs - M), one running maximum M serves pages of
 // any scale, and sum_j w_j / vs is the softmax's denominator.  M is raised (and O rescaled) only when a
@@ -27,10 +30,12 @@
 // the order of the ranges: results do not depend on timing.
 #include "common.cuh"
 #include "gqa_fp8.cuh"
+#include "sm100.cuh"
 
 namespace {
 
 using hk::GqaArgs;
+namespace sm100 = hk::sm100;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
@@ -41,8 +46,11 @@ constexpr int kRangeUnits = 16;     // units below which a range is not worth a 
 
 // CTAs that an SM holds (by registers: 128 threads of at most 96, 128, 168 or 255).
 constexpr int ctas_per_sm(int d, int nt) {
-  return d * nt <= 64 ? 5 : d * nt <= 128 ? 4 : d * nt <= 384 ? 3 : 2;
+  return d == 256 ? 2 : d * nt <= 64 ? 5 : d * nt <= 128 ? 4 : d * nt <= 384 ? 3 : 2;
 }
+// Chunks a warp keeps in flight: what 200 KB of shared memory an SM hold.
+constexpr int stages(int d, int nt) { return 200 * 1024 / (ctas_per_sm(d, nt) * kWarps * 32 * d); }
+constexpr int kLook = 16;           // chunks whose pages and scales are looked up at once
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -123,52 +131,58 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-__device__ __forceinline__ uint4 ld_once(const void* p) {
-  uint4 u;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
-  return u;
+// Where fragments lie.  A chunk's 16 tokens x D bytes are 16 D / 128 lines of 128 bytes, 16-byte part p of line y
+// stored at part p ^ (y & 7).  K: thread (r, c) reads parts k_part(c, i) of tokens r and r + 8, 4 k steps
+// each; V: 16 bytes (8 at dim 64) at v_dim(r, 4 i) of tokens 2c, 2c + 1, 2c + 8, 2c + 9.
+template <int D>
+__device__ __forceinline__ int k_part(int c, int i) {  // of a token's D / 16
+  return D == 64 ? c : D == 128 ? 2 * c + i : (i >> 1) * 8 + (c & 1) + (c >> 1) * 4 + (i & 1) * 2;
 }
-__device__ __forceinline__ uint2 ld_once8(const void* p) {
-  uint2 u;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
-  return u;
-}
-
 template <int D>
 __device__ __forceinline__ int v_dim(int r, int w) {
   return D == 64 ? r * 8 + 4 * w : (w >> 2) * 128 + r * 16 + (w & 3) * 4;
 }
-
-// K of 16 tokens as this thread's fragments hold it: tokens r and r + 8; word 4 i + m: dims 64 i + 16 c + 4 m ...
+// Address of byte 16 part of token t in a chunk.
 template <int D>
-__device__ __forceinline__ void load_k(uint32_t (&x)[2][D / 16], const uint8_t* k, int r, int c) {
+__device__ __forceinline__ const uint8_t* part_of(const uint8_t* chunk, int t, int part) {
+  const int at = t * (D / 16) + part, line = at >> 3;
+  return chunk + line * 128 + (((at & 7) ^ (line & 7)) << 4);
+}
+
+template <int D>
+__device__ __forceinline__ void read_k(uint32_t (&x)[2][D / 16], const uint8_t* chunk, int r, int c) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
-      const uint4 u = ld_once(k + (r + 8 * h) * D + i * 64 + c * 16);
+      const uint4 u = *reinterpret_cast<const uint4*>(part_of<D>(chunk, r + 8 * h, k_part<D>(c, i)));
       x[h][4 * i] = u.x, x[h][4 * i + 1] = u.y, x[h][4 * i + 2] = u.z, x[h][4 * i + 3] = u.w;
     }
 }
 
-// V of 16 tokens: tokens 2c, 2c + 1, 2c + 8, 2c + 9; word w: dims v_dim(r, w) ...
 template <int D>
-__device__ __forceinline__ void load_v(uint32_t (&x)[4][D / 32], const uint8_t* v, int r, int c) {
+__device__ __forceinline__ void read_v(uint32_t (&x)[4][D / 32], const uint8_t* chunk, int r, int c) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint8_t* p = v + (2 * c + (j & 1) + 8 * (j >> 1)) * D;
+    const int t = 2 * c + (j & 1) + 8 * (j >> 1);
     if (D == 64) {
-      const uint2 u = ld_once8(p + r * 8);
+      const uint2 u = *reinterpret_cast<const uint2*>(part_of<D>(chunk, t, r >> 1) + (r & 1) * 8);
       x[j][0] = u.x, x[j][1] = u.y;
     } else {
 #pragma unroll
       for (int i = 0; i < D / 128; ++i) {
-        const uint4 u = ld_once(p + i * 128 + r * 16);
+        const uint4 u = *reinterpret_cast<const uint4*>(part_of<D>(chunk, t, i * 8 + r));
         x[j][4 * i] = u.x, x[j][4 * i + 1] = u.y, x[j][4 * i + 2] = u.z, x[j][4 * i + 3] = u.w;
       }
     }
   }
 }
+
+// What the chunks' loop needs of a chunk: its scales and first token.
+struct Look {
+  float kf, lsv, isv;  // ks * scale * log2 e, log2 vs, 1 / vs
+  int p0;
+};
 
 // A warp's running state: 8 NT query rows (columns 2c, 2c + 1 of each N tile in this thread).
 template <int D, int NT>
@@ -288,23 +302,39 @@ __device__ __forceinline__ int64_t block_excl_scan(int64_t v, int64_t* sums, int
 
 template <int D, int NT>
 constexpr int split_smem() {
-  return kWarps / 2 * NT * (D / 16) * 32 * 16;  // O of half the warps
+  constexpr int ring = kWarps * stages(D, NT) * 32 * D, joined = kWarps / 2 * NT * (D / 16) * 32 * 16;  // O of half the warps
+  static_assert(stages(D, NT) >= 2 && stages(D, NT) <= kLook && joined <= ring, "ring");
+  return ring + 1024;  // lines are swizzled from 1 KB boundaries
 }
 
 template <int D, int NT, bool kSparse>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel(SplitArgs s) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel(SplitArgs s, const __grid_constant__ CUtensorMap kmap,
+                                                                                     const __grid_constant__ CUtensorMap vmap) {
   constexpr int R = 8 * NT;
-  extern __shared__ __align__(16) uint8_t dyn[];
-  float4* o_s = reinterpret_cast<float4*>(dyn);  // [kWarps / 2][NT * D / 16][32]
+  extern __shared__ uint8_t dyn_raw[];
+  uint8_t* dyn = dyn_raw + (1024 - (__cvta_generic_to_shared(dyn_raw) & 1023)) % 1024;
+  constexpr int S = stages(D, NT);
+  float4* o_s = reinterpret_cast<float4*>(dyn);  // [kWarps / 2][NT * D / 16][32], over the ring once it is read
   __shared__ __align__(16) uint2 q_s[NT * (D / 16) * 32];
   __shared__ float rowf_s[R], m_s[kWarps][R], l_s[kWarps][R];
   __shared__ int pos_s[R];
   __shared__ int64_t scan_s[kWarps];
   __shared__ int64_t at_s;
   __shared__ int item_s;
+  __shared__ int32_t line_s[kWarps][2 * kLook];  // first 128-byte line of a chunk in the cache, -1: not to be read
+  __shared__ __align__(8) uint64_t full_s[kWarps][S];
+  __shared__ volatile int stop_s[kWarps];  // a wait of this warp ran out: it asks for no more
+  __shared__ __align__(16) Look look_s[kWarps][2 * kLook];
   const GqaArgs& a = s.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int G = a.kv_heads, group = s.group;
+  if (tid == 0) {
+    for (int i = 0; i < kWarps; ++i) stop_s[i] = 0;
+    for (int i = 0; i < kWarps * S; ++i) sm100::mbar_init(sm100::smem_u32(&full_s[0][0] + i), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  uint32_t asked = 0, taken = 0;  // chunks this warp has asked for and read, over all its problems
+  // (the barriers are seen by all after the scan's first __syncthreads)
 
   // This CTA's range of units, and the item it begins in.
   int64_t total = 0;
@@ -377,7 +407,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) {
           const int d = lane * (D / 32) + e;
-          const int k = (d / 64) * 4 + (d % 16) / 4, cc = (d % 64) / 16;
+          const int part = d / 16, half = D == 256 ? part & 7 : part;  // the inverse of k_part
+          const int cc = D == 64 ? part : D == 128 ? part >> 1 : (half & 1) | (half >> 2) << 1;
+          const int i = D == 64 ? 0 : D == 128 ? part & 1 : (part >> 3) * 2 + (half >> 1 & 1);
+          const int k = i * 4 + (d % 16) / 4;
           reinterpret_cast<__half*>(q_s + ((n >> 3) * (D / 16) + k) * 32 + (n & 7) * 4 + cc)[d & 3] = __float2half_rn(f[e] * mul);
         }
         if (lane == 0) {
@@ -401,20 +434,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
         for (int j = 0; j < D / 16; ++j) st.o[j][n][0] = st.o[j][n][1] = st.o[j][n][2] = st.o[j][n][3] = 0.f;
       }
 
-      // This warp's chunks: tokens tok0 + 16 warp + 128 i.  Each lane looks up the page and the scales of one
-      // of the next 32.
+      // This warp's chunks: tokens tok0 + 16 warp + kUnit e.
       const int32_t* row_bt = a.bt + (int64_t)lane_b * a.bt_stride;
       const int32_t* list = kSparse ? a.blocks + ((int64_t)x.t0 * G + g) * a.top : nullptr;
       const int nchunk = tok1 > tok0 + 16 * warp ? (tok1 - tok0 - 16 * warp + kUnit - 1) / kUnit : 0;
-      for (int base = 0; base < nchunk; base += 32) {
-        int64_t offset = -1;  // of the chunk in the cache; -1: not to be read
-        int p0 = 0;           // its first token, in the lane
-        float kf = 0.f, vs = 1.f;
-        if (base + lane < nchunk) {
-          const int j = tok0 + 16 * warp + kUnit * (base + lane);
-          const int idx = j / a.page_size;
+      auto look = [&](int e0) {  // pages and scales of chunks e0 .. e0 + kLook - 1, a lane each
+        if (lane < kLook && e0 + lane < nchunk) {
+          int32_t line = -1;
+          Look y = {0.f, 0.f, 1.f, 0};
+          const int j = tok0 + 16 * warp + kUnit * (e0 + lane);
+          const int idx = j / a.page_size, r16 = j - idx * a.page_size;
           int blk = idx;
-          const int r16 = j - idx * a.page_size;
           if (kSparse) {
             blk = list[idx];
             const int before = idx > 0 ? list[idx - 1] : -1;
@@ -424,51 +454,72 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
             }
           }
           if (blk >= 0) {
-            p0 = blk * a.page_size + r16;
+            y.p0 = blk * a.page_size + r16;
             const int page = blk < a.bt_stride ? row_bt[blk] : -1;
             if (page <= 0 || page >= a.num_pages) {
               hk_flag(a.err, hk::kErrAttnPage, (unsigned)lane_b);
             } else {
-              offset = (((int64_t)page * G + g) * a.page_size + r16) * D;
-              kf = a.ks[(int64_t)page * G + g] * (a.scale * kLog2e);
-              vs = fmaxf(a.vs[(int64_t)page * G + g], 7.8886090522101181e-31f);
+              const int64_t at = (int64_t)page * G + g;
+              line = (int32_t)((at * a.page_size + r16) * D / 128);
+              y.kf = a.ks[at] * (a.scale * kLog2e);
+              const float vs = fmaxf(a.vs[at], 7.8886090522101181e-31f);
+              y.lsv = log2f(vs), y.isv = 1.f / vs;
             }
           }
+          line_s[warp][(e0 + lane) % (2 * kLook)] = line;
+          look_s[warp][(e0 + lane) % (2 * kLook)] = y;
         }
-        const float lsv = log2f(vs), isv = 1.f / vs;
-        const int m = min(32, nchunk - base);
-        // K of the next chunk is asked for once this one's scores are computed, V once its product is: one
-        // chunk in registers, and the loads of the next in flight behind the rest of the step.
-        uint32_t k[2][D / 16], v[4][D / 32];
-        int64_t off = __shfl_sync(0xffffffffu, offset, 0);
-        if (off >= 0) load_k<D>(k, a.kc + off, r, c), load_v<D>(v, a.vc + off, r, c);
+        __syncwarp();
+      };
+      uint8_t* ring = dyn + warp * (S * 32 * D);
+      auto ask = [&](int e) {
+        const int line = e < nchunk ? line_s[warp][e % (2 * kLook)] : -1;
+        if (line < 0 || stop_s[warp]) return;
+        if (lane == 0) {
+          const uint32_t bar = sm100::smem_u32(&full_s[warp][asked % S]), dst = sm100::smem_u32(ring + asked % S * (32 * D));
+          sm100::mbar_expect_tx(bar, 32 * D);
+          sm100::tma_load_2d(dst, &kmap, bar, 0, line);
+          sm100::tma_load_2d(dst + 16 * D, &vmap, bar, 0, line);
+        }
+        ++asked;
+      };
+      look(0);
+      look(kLook);
 #pragma unroll 1
-        for (int e = 0; e < m; ++e) {
-          int64_t next = __shfl_sync(0xffffffffu, offset, min(e + 1, 31));
-          if (e + 1 >= m) next = -1;
-          const int p = __shfl_sync(0xffffffffu, p0, e);
-          const float fk = __shfl_sync(0xffffffffu, kf, e), fl = __shfl_sync(0xffffffffu, lsv, e),
-                      fi = __shfl_sync(0xffffffffu, isv, e);
-          const bool edge = p + 15 > pos_min;
+      for (int e = 0; e < S - 1; ++e) ask(e);
+#pragma unroll 1
+      for (int e = 0; e < nchunk; ++e) {
+        if (e > 0 && e % kLook == 0) look(e + kLook);
+        ask(e + S - 1);  // into the stage that the step before has read
+        if (line_s[warp][e % (2 * kLook)] < 0 || taken == asked) continue;
+        const Look y = look_s[warp][e % (2 * kLook)];
+        const bool ok = __all_sync(0xffffffffu, sm100::mbar_wait(sm100::smem_u32(&full_s[warp][taken % S]), taken / S & 1,
+                                                                 &stop_s[warp], a.err, 0x60));
+        const uint8_t* mine = ring + taken % S * (32 * D);
+        ++taken;
+        if (ok) {
+          const bool edge = y.p0 + 15 > pos_min;
           float sc[NT][4];
           uint32_t pb[NT][2];
-          if (off >= 0) scores<D, NT>(sc, k, q_s, lane);
-          if (next >= 0) load_k<D>(k, a.kc + next, r, c);
-          if (off >= 0) {
-            weigh<D, NT>(st, sc, pb, rowf, fk, fl, fi, edge, p, pos_s, lane);
-            if (edge) {  // tokens past the lane's end may hold anything, NaN codes among it
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (p + 2 * c + (j & 1) + 8 * (j >> 1) >= len) {
-#pragma unroll
-                  for (int w = 0; w < D / 32; ++w) v[j][w] = 0;
-                }
-            }
-            values<D, NT>(st, v, pb);
+          {
+            uint32_t k[2][D / 16];
+            read_k<D>(k, mine, r, c);
+            scores<D, NT>(sc, k, q_s, lane);
           }
-          if (next >= 0) load_v<D>(v, a.vc + next, r, c);
-          off = next;
+          weigh<D, NT>(st, sc, pb, rowf, y.kf, y.lsv, y.isv, edge, y.p0, pos_s, lane);
+          uint32_t v[4][D / 32];
+          read_v<D>(v, mine + 16 * D, r, c);
+          if (edge) {  // tokens past the lane's end may hold anything, NaN codes among it
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (y.p0 + 2 * c + (j & 1) + 8 * (j >> 1) >= len) {
+#pragma unroll
+                for (int w = 0; w < D / 32; ++w) v[j][w] = 0;
+              }
+          }
+          values<D, NT>(st, v, pb);
         }
+        __syncwarp();
       }
 
       // Join the warps: maxima through shared memory, then O pairwise (4 + 4, 2 + 2, 1 + 1).
@@ -551,6 +602,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
             }
           }
       }
+      // O lay where the next copies go: order those writes before them.
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (starts && !ends) rec.item = i, rec.sub = sub;
       if (!starts && ends) rec.ends = 1;
       u += last - first;
@@ -631,7 +684,12 @@ int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
   s.resident = (int)(s.resident < grid ? s.resident : grid);
   if (smem > 32 * 1024)  // set on every call: cheap, and right on every device
     HK_TRY_CUDA(cudaFuncSetAttribute(gqa_split_kernel<D, NT, kSparse>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  gqa_split_kernel<D, NT, kSparse><<<grid, kThreads, smem, stream>>>(s);
+  CUtensorMap kmap, vmap;
+  const uint64_t lines = (uint64_t)s.a.num_pages * s.a.kv_heads * s.a.page_size * D / 128;
+  HK_REQUIRE(lines <= INT32_MAX, "the cache's K and V arrays must be below 2^38 bytes each");
+  HK_TRY(hk::sm100::make_map_u8(&kmap, s.a.kc, lines, 128, 16 * D / 128));
+  HK_TRY(hk::sm100::make_map_u8(&vmap, s.a.vc, lines, 128, 16 * D / 128));
+  gqa_split_kernel<D, NT, kSparse><<<grid, kThreads, smem, stream>>>(s, kmap, vmap);
   HK_TRY_LAUNCH("gqa_split_kernel");
   if (grid > 1) {
     gqa_merge_kernel<D, NT, kSparse><<<dim3(grid, NT), 256, 0, stream>>>(s, grid);
