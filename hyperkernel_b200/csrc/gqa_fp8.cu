@@ -41,8 +41,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = kWarps * 16;  // tokens
 constexpr int kMaxCtasPerSm = 5;
-constexpr int kWaves = 4;           // ranges for each resident CTA, when there is work for them
-constexpr int kRangeUnits = 16;     // units below which a range is not worth a CTA's start
 
 // CTAs that an SM holds (by registers: 128 threads of at most 96, 128, 168 or 255).
 constexpr int ctas_per_sm(int d, int nt) {
@@ -67,7 +65,6 @@ struct SplitArgs {
   int32_t is_f16;
   int32_t group, tiles_max;
   int32_t items;  // lanes (dense) or rows (sparse)
-  int32_t resident;  // CTAs that run at once
   Rec* rec;       // [grid]
   float* part;    // [grid][2][R * D + 2 R]
 };
@@ -112,6 +109,14 @@ __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same onto zero.
+__device__ __forceinline__ void mma_f16_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Four e4m3 bytes as two fp16 pairs (exact).
 __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
@@ -142,36 +147,69 @@ template <int D>
 __device__ __forceinline__ int v_dim(int r, int w) {
   return D == 64 ? r * 8 + 4 * w : (w >> 2) * 128 + r * 16 + (w & 3) * 4;
 }
-// Address of byte 16 part of token t in a chunk.
+// Offset of 16-byte part `part` of token t in a chunk.
 template <int D>
-__device__ __forceinline__ const uint8_t* part_of(const uint8_t* chunk, int t, int part) {
+__device__ __forceinline__ uint32_t part_at(int t, int part) {
   const int at = t * (D / 16) + part, line = at >> 3;
-  return chunk + line * 128 + (((at & 7) ^ (line & 7)) << 4);
+  return (uint32_t)(line * 128 + (((at & 7) ^ (line & 7)) << 4));
 }
 
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
+  uint4 u;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(p));
+  return u;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t p) {
+  uint2 u;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "r"(p));
+  return u;
+}
+
+// A thread's offsets in a chunk: K parts of token r (and r + 8), V parts of its tokens 2c and 2c + 1 (and + 8).  Eight
+// tokens on is the same line pattern 8 D bytes on, but for dim 64, where the lines' parity in the swizzle turns.
 template <int D>
-__device__ __forceinline__ void read_k(uint32_t (&x)[2][D / 16], const uint8_t* chunk, int r, int c) {
+struct Offsets {
+  uint32_t k[2][D / 64], v[4][D == 64 ? 1 : D / 128];
+  __device__ __forceinline__ Offsets(int r, int c) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) k[h][i] = part_at<D>(r + (D == 64 ? 8 * h : 0), k_part<D>(c, i)) + (D == 64 ? 0 : h * 8 * D);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = 2 * c + (j & 1), up = j >> 1;
+      if (D == 64) {
+        v[j][0] = 16 * D + part_at<D>(t + 8 * up, r >> 1) + (r & 1) * 8;
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) v[j][i] = 16 * D + part_at<D>(t, i * 8 + r) + up * 8 * D;
+      }
+    }
+  }
+};
+
+template <int D>
+__device__ __forceinline__ void read_k(uint32_t (&x)[2][D / 16], uint32_t chunk, const Offsets<D>& at) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
-      const uint4 u = *reinterpret_cast<const uint4*>(part_of<D>(chunk, r + 8 * h, k_part<D>(c, i)));
+      const uint4 u = lds16(chunk + at.k[h][i]);
       x[h][4 * i] = u.x, x[h][4 * i + 1] = u.y, x[h][4 * i + 2] = u.z, x[h][4 * i + 3] = u.w;
     }
 }
 
 template <int D>
-__device__ __forceinline__ void read_v(uint32_t (&x)[4][D / 32], const uint8_t* chunk, int r, int c) {
+__device__ __forceinline__ void read_v(uint32_t (&x)[4][D / 32], uint32_t chunk, const Offsets<D>& at) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int t = 2 * c + (j & 1) + 8 * (j >> 1);
     if (D == 64) {
-      const uint2 u = *reinterpret_cast<const uint2*>(part_of<D>(chunk, t, r >> 1) + (r & 1) * 8);
+      const uint2 u = lds8(chunk + at.v[j][0]);
       x[j][0] = u.x, x[j][1] = u.y;
     } else {
 #pragma unroll
       for (int i = 0; i < D / 128; ++i) {
-        const uint4 u = *reinterpret_cast<const uint4*>(part_of<D>(chunk, t, i * 8 + r));
+        const uint4 u = lds16(chunk + at.v[j][i]);
         x[j][4 * i] = u.x, x[j][4 * i + 1] = u.y, x[j][4 * i + 2] = u.z, x[j][4 * i + 3] = u.w;
       }
     }
@@ -191,45 +229,60 @@ struct State {
   float m[NT][2], l[NT][2];
 };
 
-// S = K Q^T of one chunk: column n * 8 + 2c + (e & 1), token r + 8 (e >> 1).
+// S = K Q^T of one chunk: column n * 8 + 2c + (e & 1), token r + 8 (e >> 1).  q: this lane's B fragments, two k
+// steps to 16 bytes.  With one N tile the eight (dim 128) products are two chains, for their latency.
 template <int D, int NT>
-__device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&k)[2][D / 16], const uint2* q_s, int lane) {
+__device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&k)[2][D / 16], uint32_t q) {
+  constexpr int kChains = NT == 1 ? 2 : 1;
+  float acc[kChains][NT][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+  for (int i = 0; i < D / 16; i += 2) {
+    uint32_t a[2][4];
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    uint32_t a0, a1, a2, a3;
-    e4m3x4_to_f16x4(k[0][i], a0, a2);
-    e4m3x4_to_f16x4(k[1][i], a1, a3);
+    for (int y = 0; y < 2; ++y) {
+      e4m3x4_to_f16x4(k[0][i + y], a[y][0], a[y][2]);
+      e4m3x4_to_f16x4(k[1][i + y], a[y][1], a[y][3]);
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const uint2 b = q_s[(n * (D / 16) + i) * 32 + lane];
-      mma_f16(s[n], a0, a1, a2, a3, b.x, b.y);
+      const uint4 b = lds16(q + (n * (D / 32) + i / 2) * 512);
+      if (i == 0) mma_f16_first(acc[0][n], a[0][0], a[0][1], a[0][2], a[0][3], b.x, b.y);
+      else mma_f16(acc[0][n], a[0][0], a[0][1], a[0][2], a[0][3], b.x, b.y);
+      if (i == 0 && kChains == 2) mma_f16_first(acc[kChains - 1][n], a[1][0], a[1][1], a[1][2], a[1][3], b.z, b.w);
+      else mma_f16(acc[kChains - 1][n], a[1][0], a[1][1], a[1][2], a[1][3], b.z, b.w);
     }
   }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[n][e] = kChains == 2 ? acc[0][n][e] + acc[1][n][e] : acc[0][n][e];
 }
 
-// The scores of one chunk become weights (B fragments of P) and enter the running sums.  kf: ks * scale *
-// log2 e; lsv, isv: log2 and inverse of vs; `edge`: some token is past a row's position.
+// The scores of one chunk become weights (B fragments of P) and enter the running sums.  y: the chunk's
+// scales; `edge`: some token is past a row's position.  The running maximum starts at a finite
+// value far below any score, so that a masked score (-inf) weighs 0 with no further test.
+constexpr float kNoMax = -1e30f;
+
 template <int D, int NT>
 __device__ __forceinline__ void weigh(State<D, NT>& st, float (&s)[NT][4], uint32_t (&b)[NT][2], const float (&rowf)[NT][2],
-                                      float kf, float lsv, float isv, bool edge, int p0, const int* pos_s, int lane) {
-  const int r = lane >> 2, c = lane & 3;
-  bool over = false;
+                                      const Look& y, bool edge, const int* pos_s, int r, int c) {
+  float p[NT][4];
+  float most = -INFINITY;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float f0 = rowf[n][0] * kf, f1 = rowf[n][1] * kf;
+    const float f0 = rowf[n][0] * y.kf, f1 = rowf[n][1] * y.kf;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], e & 1 ? f1 : f0, lsv);
+    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], e & 1 ? f1 : f0, y.lsv);
     if (edge) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (p0 + r + 8 * (e >> 1) > pos_s[n * 8 + 2 * c + (e & 1)]) s[n][e] = -INFINITY;
+        if (y.p0 + r + 8 * (e >> 1) > pos_s[n * 8 + 2 * c + (e & 1)]) s[n][e] = -INFINITY;
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) over |= fmaxf(s[n][e], s[n][e + 2]) > st.m[n][e] + 8.f;
+    for (int e = 0; e < 4; ++e) p[n][e] = s[n][e] - st.m[n][e & 1];
+    most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3])));
   }
-  if (__any_sync(0xffffffffu, over)) {
+  if (__any_sync(0xffffffffu, most > 8.f)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -238,25 +291,22 @@ __device__ __forceinline__ void weigh(State<D, NT>& st, float (&s)[NT][4], uint3
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
         const float m = fmaxf(st.m[n][e], t);
-        const float f = m == -INFINITY ? 1.f : exp2_approx(st.m[n][e] - m);
+        const float f = exp2_approx(st.m[n][e] - m);
         st.m[n][e] = m;
         st.l[n][e] *= f;
+        p[n][e] = s[n][e] - m, p[n][e + 2] = s[n][e + 2] - m;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) st.o[j][n][e] *= f, st.o[j][n][e + 2] *= f;
       }
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float p[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float m = st.m[n][e & 1];
-      p[e] = exp2_approx(s[n][e] - (m == -INFINITY ? 0.f : m));
-    }
-    st.l[n][0] = fmaf(p[0] + p[2], isv, st.l[n][0]);
-    st.l[n][1] = fmaf(p[1] + p[3], isv, st.l[n][1]);
-    b[n][0] = transpose8x8(pack2<true>(p[0], p[1]));
-    b[n][1] = transpose8x8(pack2<true>(p[2], p[3]));
+    for (int e = 0; e < 4; ++e) p[n][e] = exp2_approx(p[n][e]);
+    st.l[n][0] = fmaf(p[n][0] + p[n][2], y.isv, st.l[n][0]);
+    st.l[n][1] = fmaf(p[n][1] + p[n][3], y.isv, st.l[n][1]);
+    b[n][0] = transpose8x8(pack2<true>(p[n][0], p[n][1]));
+    b[n][1] = transpose8x8(pack2<true>(p[n][2], p[n][3]));
   }
 }
 
@@ -315,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   uint8_t* dyn = dyn_raw + (1024 - (__cvta_generic_to_shared(dyn_raw) & 1023)) % 1024;
   constexpr int S = stages(D, NT);
   float4* o_s = reinterpret_cast<float4*>(dyn);  // [kWarps / 2][NT * D / 16][32], over the ring once it is read
-  __shared__ __align__(16) uint2 q_s[NT * (D / 16) * 32];
+  __shared__ __align__(16) uint4 q_s[NT * (D / 32) * 32];  // B fragments of Q: [N tile][two k steps][lane]
   __shared__ float rowf_s[R], m_s[kWarps][R], l_s[kWarps][R];
   __shared__ int pos_s[R];
   __shared__ int64_t scan_s[kWarps];
@@ -323,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   __shared__ int item_s;
   __shared__ int32_t line_s[kWarps][2 * kLook];  // first 128-byte line of a chunk in the cache, -1: not to be read
   __shared__ __align__(8) uint64_t full_s[kWarps][S];
-  __shared__ volatile int stop_s[kWarps];  // a wait of this warp ran out: it asks for no more
+  __shared__ volatile int stop_s[kWarps];  // a wait of this warp ran out
   __shared__ __align__(16) Look look_s[kWarps][2 * kLook];
   const GqaArgs& a = s.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
@@ -333,7 +383,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
     for (int i = 0; i < kWarps * S; ++i) sm100::mbar_init(sm100::smem_u32(&full_s[0][0] + i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  uint32_t asked = 0, taken = 0;  // chunks this warp has asked for and read, over all its problems
+  // The stage (and, for reads, the phase) this warp fills and reads next, and how many are filled and not yet read.
+  int fill = 0, take = 0, filled = 0;
+  uint32_t phase = 0;
+  bool dead = false;  // a wait ran out: ask for no more
+  const Offsets<D> at(r, c);
   // (the barriers are seen by all after the scan's first __syncthreads)
 
   // This CTA's range of units, and the item it begins in.
@@ -348,9 +402,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
     block_excl_scan(n, scan_s, &all);
     total += all;
   }
-  // Several ranges for each resident CTA even out what SMs get done; short problems use all CTAs once.
-  const int64_t ranges = max(min((int64_t)gridDim.x, total / kRangeUnits), min((int64_t)s.resident, total));
-  const int64_t cta = blockIdx.x;
+  // One range for each resident CTA: two to four ranges, which even out the SMs, measured 4 to 11% slower
+  // (more starts, and more partials to join).
+  const int64_t ranges = min((int64_t)gridDim.x, total), cta = blockIdx.x;
   const int64_t u0 = cta < ranges ? total * cta / ranges : 0, u1 = cta < ranges ? total * (cta + 1) / ranges : 0;
   Rec rec = {-1, 0, 0, 0};
   if (u0 < u1) {
@@ -411,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
           const int cc = D == 64 ? part : D == 128 ? part >> 1 : (half & 1) | (half >> 2) << 1;
           const int i = D == 64 ? 0 : D == 128 ? part & 1 : (part >> 3) * 2 + (half >> 1 & 1);
           const int k = i * 4 + (d % 16) / 4;
-          reinterpret_cast<__half*>(q_s + ((n >> 3) * (D / 16) + k) * 32 + (n & 7) * 4 + cc)[d & 3] = __float2half_rn(f[e] * mul);
+          reinterpret_cast<__half*>(q_s + ((n >> 3) * (D / 32) + k / 2) * 32 + (n & 7) * 4 + cc)[(k & 1) * 4 + (d & 3)] = __float2half_rn(f[e] * mul);
         }
         if (lane == 0) {
           rowf_s[n] = __uint_as_float((uint32_t)(127 - up) << 23);
@@ -428,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
       State<D, NT> st;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        st.m[n][0] = st.m[n][1] = -INFINITY;
+        st.m[n][0] = st.m[n][1] = kNoMax;
         st.l[n][0] = st.l[n][1] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) st.o[j][n][0] = st.o[j][n][1] = st.o[j][n][2] = st.o[j][n][3] = 0.f;
@@ -471,17 +525,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
         }
         __syncwarp();
       };
-      uint8_t* ring = dyn + warp * (S * 32 * D);
+      const uint32_t ring = sm100::smem_u32(dyn) + warp * (S * 32 * D), bars = sm100::smem_u32(&full_s[warp][0]);
+      const uint32_t q_frag = sm100::smem_u32(q_s + lane);
       auto ask = [&](int e) {
         const int line = e < nchunk ? line_s[warp][e % (2 * kLook)] : -1;
-        if (line < 0 || stop_s[warp]) return;
+        if (line < 0 || dead) return;
         if (lane == 0) {
-          const uint32_t bar = sm100::smem_u32(&full_s[warp][asked % S]), dst = sm100::smem_u32(ring + asked % S * (32 * D));
+          const uint32_t bar = bars + fill * 8, dst = ring + fill * (32 * D);
           sm100::mbar_expect_tx(bar, 32 * D);
           sm100::tma_load_2d(dst, &kmap, bar, 0, line);
           sm100::tma_load_2d(dst + 16 * D, &vmap, bar, 0, line);
         }
-        ++asked;
+        fill = fill + 1 == S ? 0 : fill + 1;
+        ++filled;
       };
       look(0);
       look(kLook);
@@ -491,24 +547,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
       for (int e = 0; e < nchunk; ++e) {
         if (e > 0 && e % kLook == 0) look(e + kLook);
         ask(e + S - 1);  // into the stage that the step before has read
-        if (line_s[warp][e % (2 * kLook)] < 0 || taken == asked) continue;
+        if (line_s[warp][e % (2 * kLook)] < 0 || filled == 0) continue;
         const Look y = look_s[warp][e % (2 * kLook)];
-        const bool ok = __all_sync(0xffffffffu, sm100::mbar_wait(sm100::smem_u32(&full_s[warp][taken % S]), taken / S & 1,
-                                                                 &stop_s[warp], a.err, 0x60));
-        const uint8_t* mine = ring + taken % S * (32 * D);
-        ++taken;
+        const bool ok = __all_sync(0xffffffffu, sm100::mbar_wait(bars + take * 8, phase, &stop_s[warp], a.err, 0x60));
+        const uint32_t mine = ring + take * (32 * D);
         if (ok) {
           const bool edge = y.p0 + 15 > pos_min;
           float sc[NT][4];
           uint32_t pb[NT][2];
           {
             uint32_t k[2][D / 16];
-            read_k<D>(k, mine, r, c);
-            scores<D, NT>(sc, k, q_s, lane);
+            read_k<D>(k, mine, at);
+            scores<D, NT>(sc, k, q_frag);
           }
-          weigh<D, NT>(st, sc, pb, rowf, y.kf, y.lsv, y.isv, edge, y.p0, pos_s, lane);
+          weigh<D, NT>(st, sc, pb, rowf, y, edge, pos_s, r, c);
           uint32_t v[4][D / 32];
-          read_v<D>(v, mine + 16 * D, r, c);
+          read_v<D>(v, mine, at);
           if (edge) {  // tokens past the lane's end may hold anything, NaN codes among it
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -519,6 +573,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
           }
           values<D, NT>(st, v, pb);
         }
+        dead |= !ok;
+        --filled;
+        if (++take == S) take = 0, phase ^= 1;
         __syncwarp();
       }
 
@@ -539,14 +596,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = n * 8 + 2 * c + e;
-          float m = -INFINITY, l = 0.f;
+          float m = kNoMax, l = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) m = fmaxf(m, m_s[w][row]);
-          const float mm = m == -INFINITY ? 0.f : m;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) l += l_s[w][row] * exp2_approx(m_s[w][row] - mm);
+          for (int w = 0; w < kWarps; ++w) l += l_s[w][row] * exp2_approx(m_s[w][row] - m);
           top[n][e] = m, sum[n][e] = l;
-          const float f = exp2_approx(st.m[n][e] - mm);
+          const float f = exp2_approx(st.m[n][e] - m);
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) st.o[j][n][e] *= f, st.o[j][n][e + 2] *= f;
         }
@@ -612,42 +668,97 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   if (tid == 0) s.rec[blockIdx.x] = rec;
 }
 
-// Joins the partials of the problem that CTA blockIdx.x of the split kernel began and left open; blockIdx.y
-// picks 8 of its rows.  Warp w holds row w, lanes its dims.
-template <int D, int NT, bool kSparse>
-__global__ void __launch_bounds__(256) gqa_merge_kernel(SplitArgs s, int ctas) {
-  constexpr int R = 8 * NT, P = D / 32;
-  const GqaArgs& a = s.a;
-  const Rec rec = s.rec[blockIdx.x];
-  if (rec.item < 0) return;
-  const Item x = item_of<R, kSparse>(s, rec.item, false);
-  const int g = rec.sub / x.tiles, row0 = rec.sub % x.tiles * R;
-  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), at = row0 + row;
-  if (at >= x.rows * s.group) return;
+// Joins the partials of the problems that CTAs of the split kernel began and left open (their records), row blockIdx.y of
+// each.  A warp takes one record and joins its pieces in order, a lane holding D / 32 dims; problems of many
+// pieces (one long lane) are left to all warps of the CTA together, each taking every eighth piece.
+constexpr int kMergeWarps = 8;
+constexpr int kMergeAlone = 32;  // pieces up to which one warp joins them: a few rounds of loads
+
+struct Joined {
+  float m, l;
+};
+
+template <int D, int R>
+__device__ __forceinline__ Joined join_pieces(const float* part, int row, int from, int step, int to, int lane, float (&o)[D / 32]) {
+  constexpr int P = D / 32;
   constexpr int64_t kPart = R * D + 2 * R;
-  const float* part = s.part + ((int64_t)blockIdx.x * 2 + 1) * kPart;
-  float m = part[R * D + row], l = part[R * D + R + row], o[P];
+  Joined j = {kNoMax, 0.f};
 #pragma unroll
-  for (int e = 0; e < P; ++e) o[e] = part[row * D + lane * P + e];
-  for (int i = blockIdx.x + 1; i < ctas; ++i) {
-    part = s.part + (int64_t)i * 2 * kPart;
-    const float pm = part[R * D + row], pl = part[R * D + R + row];
-    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
-    const float f = exp2_approx(m - ref), pf = exp2_approx(pm - ref);
-    m = top;
-    l = l * f + pl * pf;
+  for (int e = 0; e < P; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int i = from; i < to; i += step) {
+    const float* p = part + ((int64_t)i * 2 + (i == 0 ? 1 : 0)) * kPart;
+    const float pm = p[R * D + row], pl = p[R * D + R + row];
+    const float top = fmaxf(j.m, pm), f = exp2_approx(j.m - top), pf = exp2_approx(pm - top);
+    j.m = top;
+    j.l = j.l * f + pl * pf;
 #pragma unroll
-    for (int e = 0; e < P; ++e) o[e] = o[e] * f + part[row * D + lane * P + e] * pf;
-    if (s.rec[i].ends) break;
+    for (int e = 0; e < P; ++e) o[e] = o[e] * f + p[row * D + lane * P + e] * pf;
   }
-  const int64_t y = (int64_t)(x.t0 + at / s.group) * a.q_heads + g * s.group + at % s.group;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int e = 0; e < P; e += 2) {
-    const float lo = o[e] * inv, hi = o[e + 1] * inv;
-    *reinterpret_cast<uint32_t*>(a.out + y * D + lane * P + e) = s.is_f16 ? pack2<true>(lo, hi) : pack2<false>(lo, hi);
+  return j;
+}
+
+template <int D, int NT, bool kSparse>
+__global__ void __launch_bounds__(kMergeWarps * 32) gqa_merge_kernel(SplitArgs s, int ctas) {
+  constexpr int R = 8 * NT, P = D / 32;
+  constexpr int64_t kPart = R * D + 2 * R;
+  __shared__ float o_s[kMergeWarps][D], m_s[kMergeWarps], l_s[kMergeWarps];
+  __shared__ int pieces_s[kMergeWarps];
+  __shared__ int64_t row_s[kMergeWarps];
+  const GqaArgs& a = s.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.y;
+  const int first = blockIdx.x * kMergeWarps + warp;
+  int pieces = 0;
+  int64_t y = 0;  // (row, head) of the output
+  const Rec rec = first < ctas ? s.rec[first] : Rec{-1, 0, 0, 0};
+  if (rec.item >= 0) {
+    const Item x = item_of<R, kSparse>(s, rec.item, false);
+    const int g = rec.sub / x.tiles, at = rec.sub % x.tiles * R + row;
+    if (at < x.rows * s.group) {
+      y = (int64_t)(x.t0 + at / s.group) * a.q_heads + g * s.group + at % s.group;
+      // The last piece: the first CTA after this one in which a continued problem ends.
+      for (int base = first + 1; pieces == 0; base += 32) {
+        const unsigned hit = __ballot_sync(0xffffffffu, base + lane >= ctas || s.rec[min(base + lane, ctas - 1)].ends);
+        if (hit) pieces = min(base + __ffs(hit) - 1, ctas - 1) - first + 1;
+      }
+    }
   }
-  if (lane == 0) a.lse[y] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
+  if (pieces > 0 && pieces <= kMergeAlone) {
+    float o[P];
+    const Joined j = join_pieces<D, R>(s.part + (int64_t)first * 2 * kPart, row, 0, 1, pieces, lane, o);
+    const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+#pragma unroll
+    for (int e = 0; e < P; e += 2)
+      *reinterpret_cast<uint32_t*>(a.out + y * D + lane * P + e) =
+          s.is_f16 ? pack2<true>(o[e] * inv, o[e + 1] * inv) : pack2<false>(o[e] * inv, o[e + 1] * inv);
+    if (lane == 0) a.lse[y] = j.l == 0.f ? -INFINITY : fmaf(j.m, kLn2, logf(j.l));
+  }
+  if (lane == 0) pieces_s[warp] = pieces, row_s[warp] = y;
+  __syncthreads();
+  for (int w = 0; w < kMergeWarps; ++w) {
+    if (pieces_s[w] <= kMergeAlone) continue;
+    float o[P];
+    const Joined j = join_pieces<D, R>(s.part + (int64_t)(blockIdx.x * kMergeWarps + w) * 2 * kPart, row, warp, kMergeWarps, pieces_s[w], lane, o);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < P; ++e) o_s[warp][lane * P + e] = o[e];
+    if (lane == 0) m_s[warp] = j.m, l_s[warp] = j.l;
+    __syncthreads();
+    if (tid < D / 2) {
+      float top = kNoMax, sum = 0.f, v[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < kMergeWarps; ++e) top = fmaxf(top, m_s[e]);
+#pragma unroll
+      for (int e = 0; e < kMergeWarps; ++e) {
+        const float f = exp2_approx(m_s[e] - top);
+        sum += l_s[e] * f;
+        v[0] = fmaf(o_s[e][2 * tid], f, v[0]), v[1] = fmaf(o_s[e][2 * tid + 1], f, v[1]);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<uint32_t*>(a.out + row_s[w] * D + 2 * tid) = s.is_f16 ? pack2<true>(v[0] * inv, v[1] * inv) : pack2<false>(v[0] * inv, v[1] * inv);
+      if (tid == 0) a.lse[row_s[w]] = sum == 0.f ? -INFINITY : fmaf(top, kLn2, logf(sum));
+    }
+  }
 }
 
 int check(const char* name, const GqaArgs& a, int32_t dtype) {
@@ -677,11 +788,8 @@ size_t part_floats(int nt, int dim) { return (size_t)8 * nt * dim + 16 * nt; }
 template <int D, int NT, bool kSparse>
 int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
   constexpr int smem = split_smem<D, NT>();
-  s.resident = hk::sm_count() * ctas_per_sm(D, NT);
-  const int64_t wide = units / kRangeUnits < (int64_t)s.resident * kWaves ? units / kRangeUnits : (int64_t)s.resident * kWaves;
-  const int64_t once = units < s.resident ? units : s.resident;
-  const int grid = (int)(wide > once ? wide : once);
-  s.resident = (int)(s.resident < grid ? s.resident : grid);
+  const int64_t resident = hk::sm_count() * ctas_per_sm(D, NT);
+  const int grid = (int)(units < resident ? units : resident);
   if (smem > 32 * 1024)  // set on every call: cheap, and right on every device
     HK_TRY_CUDA(cudaFuncSetAttribute(gqa_split_kernel<D, NT, kSparse>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   CUtensorMap kmap, vmap;
@@ -692,7 +800,7 @@ int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
   gqa_split_kernel<D, NT, kSparse><<<grid, kThreads, smem, stream>>>(s, kmap, vmap);
   HK_TRY_LAUNCH("gqa_split_kernel");
   if (grid > 1) {
-    gqa_merge_kernel<D, NT, kSparse><<<dim3(grid, NT), 256, 0, stream>>>(s, grid);
+    gqa_merge_kernel<D, NT, kSparse><<<dim3((grid + kMergeWarps - 1) / kMergeWarps, 8 * NT), kMergeWarps * 32, 0, stream>>>(s, grid);
     HK_TRY_LAUNCH("gqa_merge_kernel");
   }
   return HK_OK;
@@ -707,7 +815,7 @@ int launch(const GqaArgs& a, int32_t dtype, int64_t rows, int64_t units, void* w
   s.group = a.q_heads / a.kv_heads;
   s.items = kSparse ? a.num_tokens : a.num_lanes;
   s.rec = (Rec*)workspace;
-  s.part = (float*)((uint8_t*)workspace + (size_t)hk::sm_count() * kMaxCtasPerSm * kWaves * sizeof(Rec));
+  s.part = (float*)((uint8_t*)workspace + (size_t)hk::sm_count() * kMaxCtasPerSm * sizeof(Rec));
   const int nt = n_tiles(rows * s.group, a.dim);
   switch (a.dim * 8 + nt) {
 #define HK_GQA(D, NT) \
@@ -740,7 +848,7 @@ size_t hk_gqa_fp8_workspace_size(int32_t num_tokens, int32_t q_heads, int32_t kv
     const size_t part = ctas_per_sm(head_dim, n) * 2 * part_floats(n, head_dim) * sizeof(float);
     most = most > part ? most : part;
   }
-  return (size_t)hk::sm_count() * kWaves * (kMaxCtasPerSm * sizeof(Rec) + most);
+  return (size_t)hk::sm_count() * (kMaxCtasPerSm * sizeof(Rec) + most);
 }
 
 int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache, const uint8_t* v_cache,

@@ -9,16 +9,20 @@
 // blocks are always read; the rest of top_blocks go to the highest scores, equal ones to the lower
 // block.
 //
-// One CTA per (row, KV head): scores to the workspace as keys whose unsigned order is the
-// scores' order, a radix select for the top_blocks-th key (8 bits a pass), and one ordered pass
-// that writes the chosen indices rising.
+// Two kernels.  The first spreads the scores over CTAs of 256 blocks (a centroid is read by dim / 16
+// lanes, 16 bytes each, and dotted by dp4a) and leaves them in the workspace as keys whose unsigned
+// order is the scores' order: bound by reading the centroids.  The second has one CTA per (row, KV head),
+// whose threads hold the keys in registers and find the lowest chosen key bit by bit from the
+// first bit in which the keys differ: counts by warp reductions, so that equal leading bits, which
+// scores have, cost no contention.  One scan then places the chosen indices in rising order.
 #include "common.cuh"
 #include "gqa_fp8.cuh"
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kScoreThreads = 128;
+constexpr int kScoreBlocks = 256;  // per CTA
+constexpr int kHold = 16;          // keys a thread of the second kernel holds
 
 struct SelectArgs {
   const uint16_t* q;
@@ -42,40 +46,37 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
+// Blocks in sight of row t; 0 when they pass the call's max_kv_len.
+__device__ __forceinline__ int blocks_of(const SelectArgs& a, int t) {
+  const int pos = a.positions[t];
+  const int n = pos < 0 ? 0 : pos / a.page_size + 1;
+  return n <= a.max_blocks ? n : 0;
+}
+
 template <bool kF16>
-__global__ void __launch_bounds__(kThreads) gqa_select_kernel(SelectArgs a) {
-  __shared__ float u[256];
+__global__ void __launch_bounds__(kScoreThreads) gqa_score_kernel(SelectArgs a) {
+  __shared__ float warp_max[kScoreThreads / 32];
   __shared__ __align__(16) int8_t c8[256];
-  __shared__ float warp_max[kWarps];
-  __shared__ int hist[256];
-  __shared__ int warp_sum[2][kWarps];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_rank;
   const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (t >= a.cu[a.num_lanes]) return;
-  const int pos = a.positions[t];
-  int32_t* list = a.blocks + ((int64_t)t * a.kv_heads + g) * a.top;
-  int n = pos < 0 ? 0 : pos / a.page_size + 1;
-  if (n > a.max_blocks) {
-    if (tid == 0) hk_flag(a.err, hk::kErrPosition, (unsigned)t);
-    n = 0;
-  }
-  if (n <= a.top) {
-    for (int i = tid; i < a.top; i += kThreads) list[i] = i < n ? i : -1;
-    return;
-  }
+  const int n = blocks_of(a, t), from = blockIdx.z * kScoreBlocks, to = min(n - a.local, from + kScoreBlocks);
+  if (n <= a.top || from >= to) return;
   const int b = hk::lane_of_row(a.cu, a.num_lanes, t);
   const int group = a.q_heads / a.kv_heads;
-  float mine = 0.f;
-  if (tid < a.dim) {
+  float u[2] = {0.f, 0.f}, mine = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = tid + k * kScoreThreads;
+    if (d >= a.dim) continue;
     double sum = 0.0;
+#pragma unroll 4
     for (int h = 0; h < group; ++h) {
-      const uint16_t w = a.q[t * a.q_stride + (int64_t)(g * group + h) * a.dim + tid];
+      const uint16_t w = a.q[t * a.q_stride + (int64_t)(g * group + h) * a.dim + d];
       sum += (double)(kF16 ? __half2float(*reinterpret_cast<const __half*>(&w)) : bf16_bits_to_f32(w));
     }
-    u[tid] = (float)sum;
-    mine = fabsf(u[tid]);
-    if (!(mine < INFINITY)) mine = INFINITY;
+    u[k] = (float)sum;
+    const float v = fabsf(u[k]);
+    mine = v < INFINITY ? fmaxf(mine, v) : INFINITY;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
@@ -83,92 +84,128 @@ __global__ void __launch_bounds__(kThreads) gqa_select_kernel(SelectArgs a) {
   __syncthreads();
   float m = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_max[w]);
-  // A row with a value that is not finite scores 0 everywhere: its blocks are the first ones.
+  for (int w = 0; w < kScoreThreads / 32; ++w) m = fmaxf(m, warp_max[w]);
+  // A row with a value that is not finite scores 0 everywhere.
   const float r = m > 0.f && m < INFINITY ? __fdiv_rn(127.f, m) : 0.f;
-  if (tid < a.dim) c8[tid] = r > 0.f ? (int8_t)rintf(__fmul_rn(u[tid], r)) : (int8_t)0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = tid + k * kScoreThreads;
+    if (d < a.dim) c8[d] = r > 0.f ? (int8_t)rintf(__fmul_rn(u[k], r)) : (int8_t)0;
+  }
   __syncthreads();
 
+  const int vec = a.dim / 16, sub = lane % vec;  // 4, 8 or 16 lanes per centroid
+  const int4 y = reinterpret_cast<const int4*>(c8)[sub];
   uint32_t* keys = a.keys + ((int64_t)t * a.kv_heads + g) * a.max_blocks;
-  const int vec = a.dim / 16;  // 16-byte parts of a centroid
-  for (int i = tid; i < n; i += kThreads) {
-    uint32_t key;
-    if (i < a.sink || i >= n - a.local) {
-      key = 0xffffffffu;
-    } else {
-      const int page = i < a.bt_stride ? a.bt[(int64_t)b * a.bt_stride + i] : -1;
-      if (page <= 0 || page >= a.num_pages) {
-        hk_flag(a.err, hk::kErrAttnPage, (unsigned)b);
-        key = 0;
-      } else {
-        const int64_t at = (int64_t)page * a.kv_heads + g;
-        const int4* cen = reinterpret_cast<const int4*>(a.centroids + at * a.dim);
-        int dot = 0;
-        for (int v = 0; v < vec; ++v) {
-          const int4 x = cen[v], y = reinterpret_cast<const int4*>(c8)[v];
-          dot = __dp4a(x.x, y.x, dot), dot = __dp4a(x.y, y.y, dot);
-          dot = __dp4a(x.z, y.z, dot), dot = __dp4a(x.w, y.w, dot);
-        }
-        key = order_key(__fadd_rn(__fmul_rn((float)dot, a.centroid_scale[at]), 0.f));  // -0 becomes 0
-        key = min(key, 0xfffffffeu);
-      }
+  const int per = kScoreThreads / vec;
+#pragma unroll 4
+  for (int base = from; base < to; base += per) {
+    const int i = base + tid / vec;
+    int page = -1;
+    if (i < to && i < a.bt_stride) page = a.bt[(int64_t)b * a.bt_stride + i];
+    const bool ok = page > 0 && page < a.num_pages;
+    const int64_t at = (int64_t)(ok ? page : 0) * a.kv_heads + g;
+    const int4 x = reinterpret_cast<const int4*>(a.centroids + at * a.dim)[sub];
+    const float f = a.centroid_scale[at];
+    int dot = __dp4a(x.x, y.x, __dp4a(x.y, y.y, __dp4a(x.z, y.z, __dp4a(x.w, y.w, 0))));
+    for (int o = 1; o < vec; o <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (sub == 0 && i < to) {
+      if (!ok && i >= a.sink) hk_flag(a.err, hk::kErrAttnPage, (unsigned)b);
+      keys[i] = ok ? order_key(__fadd_rn(__fmul_rn((float)dot, f), 0.f)) : 0u;  // -0 becomes 0
     }
-    keys[i] = key;
   }
-  if (tid == 0) s_prefix = 0, s_rank = a.top;
-  // The top-th largest key, from its highest 8 bits down: s_rank = how many of the keys that
-  // share the prefix are wanted.
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    hist[tid] = 0;
-    __syncthreads();
-    const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int i = tid; i < n; i += kThreads) {
-      const uint32_t k = keys[i];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
-    }
-    __syncthreads();
-    // Keys at or above each bin: a scan from the highest bin down.
-    const int bin = 255 - tid, here = hist[bin];
-    int x = here;
+}
+
+// kThreads threads hold kHold keys each (`kHeld`), or read them again for every count where there are more.
+template <int kThreads, bool kHeld>
+__global__ void __launch_bounds__(kThreads) gqa_select_kernel(SelectArgs a) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ uint32_t and_s, or_s;
+  __shared__ int count_s[32];
+  __shared__ int64_t sums_s[kWarps];
+  const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (t >= a.cu[a.num_lanes]) return;
+  int32_t* list = a.blocks + ((int64_t)t * a.kv_heads + g) * a.top;
+  const int n = blocks_of(a, t);
+  if (n == 0 && a.positions[t] >= 0 && tid == 0) hk_flag(a.err, hk::kErrPosition, (unsigned)t);
+  if (n <= a.top) {
+    for (int i = tid; i < a.top; i += kThreads) list[i] = i < n ? i : -1;
+    return;
+  }
+  for (int i = tid; i < a.sink; i += kThreads) list[i] = i;
+  for (int i = tid; i < a.local; i += kThreads) list[a.top - a.local + i] = n - a.local + i;
+  const int want = a.top - a.sink - a.local, m = n - a.sink - a.local;
+  if (want == 0) return;
+  const uint32_t* keys = a.keys + ((int64_t)t * a.kv_heads + g) * a.max_blocks + a.sink;
+  // Thread tid has keys tid * per .. + per - 1.
+  const int per = (m + kThreads - 1) / kThreads, first = tid * per, mine = max(0, min(per, m - first));
+  uint32_t k[kHeld ? kHold : 1];
+  uint32_t all = 0xffffffffu, any = 0;
+  if (kHeld) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) warp_sum[0][warp] = x;
-    const int want = s_rank;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < warp; ++w) before += warp_sum[0][w];
-    const int above = before + x - here;
-    if (above < want && above + here >= want) {
-      s_prefix = prefix | ((uint32_t)bin << shift);
-      s_rank = want - above;
-    }
-    __syncthreads();
+    for (int j = 0; j < kHold; ++j)
+      if (j < mine) k[j] = keys[first + j], all &= k[j], any |= k[j];
+  } else {
+    for (int j = 0; j < mine; ++j) all &= keys[first + j], any |= keys[first + j];
   }
-  const uint32_t cut = s_prefix;
-  const int ties = s_rank;  // keys equal to `cut` that are taken, the lower blocks first
-  int done = 0, tied = 0;
-  for (int base = 0; base < n && done < a.top; base += kThreads) {
-    const int i = base + tid;
-    const uint32_t k = i < n ? keys[i] : 0u;
-    const bool eq = i < n && k == cut, gt = i < n && k > cut;
-    const unsigned beq = __ballot_sync(0xffffffffu, eq), bgt = __ballot_sync(0xffffffffu, gt);
-    __syncthreads();
-    if (lane == 0) warp_sum[0][warp] = __popc(beq), warp_sum[1][warp] = __popc(bgt);
-    __syncthreads();
-    int eq_before = tied, gt_before = done - min(tied, ties), eq_all = tied, gt_all = gt_before;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) eq_before += warp_sum[0][w], gt_before += warp_sum[1][w];
-      eq_all += warp_sum[0][w], gt_all += warp_sum[1][w];
+  auto count = [&](uint32_t at_least) {
+    int c = 0;
+    if (kHeld) {
+#pragma unroll
+      for (int j = 0; j < kHold; ++j) c += j < mine && k[j] >= at_least;
+    } else {
+      for (int j = 0; j < mine; ++j) c += keys[first + j] >= at_least;
     }
-    const unsigned low = (1u << lane) - 1u;
-    eq_before += __popc(beq & low), gt_before += __popc(bgt & low);
-    const bool take = gt || (eq && eq_before < ties);
-    if (take) list[gt_before + min(eq_before, ties)] = i;
-    tied = eq_all;
-    done = gt_all + min(tied, ties);
+    return c;
+  };
+  if (tid < 32) count_s[tid] = 0;
+  if (tid == 0) and_s = 0xffffffffu, or_s = 0;
+  __syncthreads();
+  all = __reduce_and_sync(0xffffffffu, all), any = __reduce_or_sync(0xffffffffu, any);
+  if (lane == 0) atomicAnd(&and_s, all), atomicOr(&or_s, any);
+  __syncthreads();
+  all = and_s;
+  const uint32_t vary = all ^ or_s;
+  // The largest value that at least `want` keys reach: bits above the first varying one are common.
+  uint32_t cut = vary == 0 ? all : all & ~(0xffffffffu >> __clz(vary));
+  int reach = m;  // keys >= cut
+  for (int bit = vary == 0 ? -1 : 31 - __clz(vary); bit >= 0 && reach != want; --bit) {
+    const uint32_t tryout = cut | (1u << bit);
+    const int c = __reduce_add_sync(0xffffffffu, count(tryout));
+    if (lane == 0) atomicAdd(&count_s[bit], c);
+    __syncthreads();
+    if (count_s[bit] >= want) cut = tryout, reach = count_s[bit];
+  }
+  // All keys above the cut are taken, and of those equal to it the lower blocks, until `want` are.
+  const int above = reach == want ? count(cut) : cut == 0xffffffffu ? 0 : count(cut + 1);
+  const int equal = reach == want ? 0 : count(cut) - above;
+  const int64_t v = (int64_t)above << 32 | equal;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sums_s[warp] = x;
+  __syncthreads();
+  int64_t before = x - v, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums_s[w];
+    total += sums_s[w];
+  }
+  const int ties = want - (int)(total >> 32);
+  int gt = (int)(before >> 32), eq = (int)(uint32_t)before;
+  auto place = [&](int j, uint32_t key) {
+    const bool over = reach == want ? key >= cut : key > cut, same = reach != want && key == cut;
+    if (over || (same && eq < ties)) list[a.sink + gt + min(eq, ties)] = a.sink + first + j;
+    gt += over, eq += same;
+  };
+  if (kHeld) {
+#pragma unroll
+    for (int j = 0; j < kHold; ++j)
+      if (j < mine) place(j, k[j]);
+  } else {
+    for (int j = 0; j < mine; ++j) place(j, keys[first + j]);
   }
 }
 
@@ -213,9 +250,19 @@ int hk_gqa_select_blocks(const uint16_t* q, int64_t q_stride, const int8_t* cent
                   num_tokens, q_heads, kv_heads, head_dim, page_size, num_pages,
                   (int32_t)(((int64_t)max_kv_len + page_size - 1) / page_size), top_blocks, sink, local, blocks,
                   (uint32_t*)workspace, hk::err_word()};
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int parts = (a.max_blocks + kScoreBlocks - 1) / kScoreBlocks;
+  HK_REQUIRE(parts <= 65535, "hk_gqa_select_blocks: max_kv_len %d holds too many blocks", max_kv_len);
+  if (a.max_blocks > top_blocks) {  // else every list is the whole range
+    const dim3 grid(num_tokens, kv_heads, parts);
+    if (dtype == HK_F16) gqa_score_kernel<true><<<grid, kScoreThreads, 0, st>>>(a);
+    else gqa_score_kernel<false><<<grid, kScoreThreads, 0, st>>>(a);
+    HK_TRY_LAUNCH("gqa_score_kernel");
+  }
   const dim3 grid(num_tokens, kv_heads);
-  if (dtype == HK_F16) gqa_select_kernel<true><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
-  else gqa_select_kernel<false><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
+  if (a.max_blocks <= 256 * kHold) gqa_select_kernel<256, true><<<grid, 256, 0, st>>>(a);
+  else if (a.max_blocks <= 1024 * kHold) gqa_select_kernel<1024, true><<<grid, 1024, 0, st>>>(a);
+  else gqa_select_kernel<1024, false><<<grid, 1024, 0, st>>>(a);
   HK_TRY_LAUNCH("gqa_select_kernel");
   return HK_OK;
 }

@@ -37,9 +37,10 @@ struct NormRopeArgs {
 template <bool kF16, int LPH, bool kPairs>
 __global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(NormRopeArgs a) {
   constexpr int kGroups = 32 / LPH;  // heads side by side in a warp
-  const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int64_t t = item / a.items;
-  if (t >= a.num_tokens) return;
+  const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const uint32_t row = item / (uint32_t)a.items;
+  if (row >= (uint32_t)a.num_tokens) return;
+  const int64_t t = row;
   const int pos = a.positions[t];
   if (pos < 0) return;  // a padding row
   const int lane = threadIdx.x & 31, sub = lane % LPH, e0 = sub * 8;
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(NormRopeArgs a) 
     return;
   }
   const bool on = e0 < a.dim;
-  const int h0 = (int)(item % a.items) * (kGroups * kIters) + lane / LPH;
+  const int h0 = (int)(item - row * a.items) * (kGroups * kIters) + lane / LPH;
   const int total = a.heads[0] + a.heads[1];
 
   uint4 v[kIters];
@@ -61,16 +62,25 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(NormRopeArgs a) 
       v[i] = *reinterpret_cast<const uint4*>(a.x[w] + t * a.xs[w] + (int64_t)(h - w * a.heads[0]) * a.dim + e0);
     }
   }
-  // This lane's 8 cosines and sines; 1 and 0 outside the rotated dims.
+  // This lane's 8 cosines and sines (4 of each, twice, when neighbours pair up); 1 and 0 outside the rotated dims.
   float c[8], s[8];
   const float* line = a.table + (int64_t)pos * a.rot;
   const int half = a.rot / 2;
   const bool turned = e0 < a.rot;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int f = kPairs ? (e0 + j) / 2 : (e0 < half ? e0 + j : e0 + j - half);
-    c[j] = turned ? line[f] : 1.f;
-    s[j] = turned ? line[half + f] : 0.f;
+  for (int j = 0; j < 8; ++j) c[j] = 1.f, s[j] = 0.f;
+  if (turned) {
+    const float* f = line + (kPairs ? e0 / 2 : e0 < half ? e0 : e0 - half);
+#pragma unroll
+    for (int j = 0; j < (kPairs ? 4 : 8); j += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(f + j), y = *reinterpret_cast<const float4*>(f + half + j);
+      const float cx[4] = {x.x, x.y, x.z, x.w}, sx[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (kPairs) c[2 * e] = c[2 * e + 1] = cx[e], s[2 * e] = s[2 * e + 1] = sx[e];
+        else c[j + e] = cx[e], s[j + e] = sx[e];
+      }
+    }
   }
   const float inv_dim = 1.f / (float)a.dim;
   const int partner = e0 < half ? lane + half / 8 : lane - half / 8;  // halves form: rot % 16 == 0
@@ -86,7 +96,7 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(NormRopeArgs a) 
     for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = 1.f / sqrtf(fmaf(ss, inv_dim, a.eps));
+    const float r = rsqrtf(fmaf(ss, inv_dim, a.eps));
     float g[8];
     if (a.gain[w] != nullptr && on) {
       unpack8<kF16>(*reinterpret_cast<const uint4*>(a.gain[w] + e0), g);
@@ -143,7 +153,7 @@ extern "C" int hk_qk_norm_rope(const uint16_t* q, int64_t q_stride, const uint16
   HK_REQUIRE((q_heads == 0 || (q && q_out)) && (kv_heads == 0 || (k && k_out)) && positions && (table || rot_dim == 0),
              "hk_qk_norm_rope: null pointer");
   HK_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_gain |
-              (uintptr_t)k_gain) % 16 == 0,
+              (uintptr_t)k_gain | (uintptr_t)table) % 16 == 0,
              "hk_qk_norm_rope: buffers must be 16-byte aligned");
   HK_TRY(hk::ensure_device());
   NormRopeArgs a;
@@ -156,7 +166,7 @@ extern "C" int hk_qk_norm_rope(const uint16_t* q, int64_t q_stride, const uint16
   const int per = 32 / lph * kIters;
   a.items = (q_heads + kv_heads + per - 1) / per;
   const int64_t ctas = ((int64_t)num_tokens * a.items + kWarps - 1) / kWarps;
-  HK_REQUIRE(ctas <= INT32_MAX, "hk_qk_norm_rope: too many heads in one call");
+  HK_REQUIRE(ctas * kWarps <= INT32_MAX, "hk_qk_norm_rope: too many heads in one call");
   const cudaStream_t s = (cudaStream_t)stream;
   const bool pairs = interleaved != 0;
   if (dtype == HK_F16) {
