@@ -65,6 +65,7 @@ struct SplitArgs {
   int32_t is_f16;
   int32_t group, tiles_max;
   int32_t items;  // lanes (dense) or rows (sparse)
+  int32_t most;   // dense: query rows (rows x group) of a lane above which it is not this kernel's
   Rec* rec;       // [grid]
   float* part;    // [grid][2][R * D + 2 R]
 };
@@ -94,6 +95,7 @@ __device__ __forceinline__ Item item_of(const SplitArgs& s, int i, bool report) 
       if (report) hk_flag(a.err, hk::kErrLaneRows, (unsigned)i);
       x.rows = 0;
     }
+    if ((int64_t)x.rows * s.group > s.most) x.rows = 0;
     x.pos = 0;
     x.len = x.rows ? max(0, a.positions[t1 - 1] + 1) : 0;
   }
@@ -783,6 +785,12 @@ int n_tiles(int64_t rows, int dim) {
   return (int)(n < most ? n : most);
 }
 
+// Query rows (rows x heads of a group) of a lane above which the tcgen05 kernel takes it: two 32-row tiles of
+// the split kernel, which read the cache twice, against one of its 256-row tiles.
+constexpr int32_t kFewRows = 64;
+
+size_t split_workspace(int64_t rows, int dim);
+
 size_t part_floats(int nt, int dim) { return (size_t)8 * nt * dim + 16 * nt; }
 
 template <int D, int NT, bool kSparse>
@@ -807,10 +815,10 @@ int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
 }
 
 template <bool kSparse>
-int launch(const GqaArgs& a, int32_t dtype, int64_t rows, int64_t units, void* workspace, cudaStream_t stream) {
+int launch(const GqaArgs& a, int32_t dtype, int64_t rows, int64_t units, int32_t most, void* workspace, cudaStream_t stream) {
   SplitArgs s;
   s.a = a;
-  s.a.err = hk::err_word();
+  s.most = most;
   s.is_f16 = dtype == HK_F16;
   s.group = a.q_heads / a.kv_heads;
   s.items = kSparse ? a.num_tokens : a.num_lanes;
@@ -838,17 +846,29 @@ int launch(const GqaArgs& a, int32_t dtype, int64_t rows, int64_t units, void* w
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-size_t hk_gqa_fp8_workspace_size(int32_t num_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
-  if (num_tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
-  const int nt = n_tiles((int64_t)num_tokens * (q_heads / kv_heads > 0 ? q_heads / kv_heads : 1), head_dim);
+// Bytes of the split kernel's records and partials for problems of up to `rows` query rows.
+size_t split_workspace(int64_t rows, int head_dim) {
+  const int nt = n_tiles(rows, head_dim);
   size_t most = 0;  // over the tile counts that a call with these sizes can pick
   for (int n = 1; n <= nt; ++n) {
     const size_t part = ctas_per_sm(head_dim, n) * 2 * part_floats(n, head_dim) * sizeof(float);
     most = most > part ? most : part;
   }
-  return (size_t)hk::sm_count() * (kMaxCtasPerSm * sizeof(Rec) + most);
+  return ((size_t)hk::sm_count() * (kMaxCtasPerSm * sizeof(Rec) + most) + 255) / 256 * 256;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t hk_gqa_fp8_workspace_size(int32_t num_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
+  if (num_tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
+  const int64_t rows = (int64_t)num_tokens * (q_heads / kv_heads > 0 ? q_heads / kv_heads : 1);
+  size_t bytes = split_workspace(rows, head_dim);
+  if (rows > kFewRows && hk::gqa_prefill_supported(head_dim)) bytes += (hk::gqa_prefill_workspace(head_dim) + 255) / 256 * 256;
+  return bytes;
 }
 
 int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache, const uint8_t* v_cache,
@@ -867,10 +887,20 @@ int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cach
   if (workspace == nullptr || workspace_bytes < hk_gqa_fp8_workspace_size(num_tokens, q_heads, kv_heads, head_dim))
     return hk::fail(HK_ESPACE, "hk_gqa_decode_fp8: workspace of %zu bytes is too small", workspace_bytes);
   HK_TRY(hk::ensure_device());
-  const int64_t rows = max_rows < num_tokens ? max_rows : num_tokens;
-  const int64_t tiles = rows * (q_heads / kv_heads) / 8 + 1;
+  a.err = hk::err_word();
+  const int group = q_heads / kv_heads;
+  int64_t rows = max_rows < num_tokens ? max_rows : num_tokens;
+  int32_t most = INT32_MAX;
+  if (rows * group > kFewRows && hk::gqa_prefill_supported(head_dim)) {
+    void* at = (uint8_t*)workspace + split_workspace((int64_t)num_tokens * group, head_dim);
+    HK_TRY(hk::gqa_prefill(a, dtype, kFewRows, max_kv_len, at, (cudaStream_t)stream));
+    most = kFewRows;
+    if (kFewRows / group == 0) return HK_OK;  // one row is already above it
+    rows = kFewRows / group;
+  }
+  const int64_t tiles = rows * group / 8 + 1;
   const int64_t units = (int64_t)(num_lanes < num_tokens ? num_lanes : num_tokens) * kv_heads * tiles * (max_kv_len / kUnit + 1);
-  return launch<false>(a, dtype, rows > 0 ? rows : 1, units, workspace, (cudaStream_t)stream);
+  return launch<false>(a, dtype, rows > 0 ? rows : 1, units, most, workspace, (cudaStream_t)stream);
 }
 
 int hk_gqa_sparse_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache, const uint8_t* v_cache,
@@ -892,7 +922,8 @@ int hk_gqa_sparse_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cach
   HK_TRY(hk::ensure_device());
   const int group = q_heads / kv_heads;
   const int64_t units = (int64_t)num_tokens * kv_heads * (group / 8 + 1) * ((int64_t)top_blocks * page_size / kUnit + 1);
-  return launch<true>(a, dtype, 1, units, workspace, (cudaStream_t)stream);
+  a.err = hk::err_word();
+  return launch<true>(a, dtype, 1, units, INT32_MAX, workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -39,3 +39,13 @@ __device__ __forceinline__ int lane_of_row(const int32_t* __restrict__ cu, int n
 }
 
 }  // namespace hk
+
+namespace hk {
+
+// The tcgen05 kernel for prompt chunks (gqa_prefill.cu): the lanes with more than `least` query rows (rows x
+// heads of a group) at dims 64 and 128.  `workspace`: gqa_prefill_workspace bytes.
+bool gqa_prefill_supported(int32_t dim);
+size_t gqa_prefill_workspace(int32_t dim);
+int gqa_prefill(const GqaArgs& a, int32_t dtype, int32_t least, int64_t max_kv_len, void* workspace, cudaStream_t stream);
+
+}  // namespace hk
