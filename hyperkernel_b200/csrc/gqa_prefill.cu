@@ -18,7 +18,8 @@
 // equal contiguous range of them.  Problems cut by a range's end leave fp32 partials, two at
 // most for each SM, which the merge kernel joins in the order of the ranges.
 //
-// Roles (16 warps): 0-3 and 4-7 softmax of the two halves, 8-11 conversion, 12 product issue, 13 TMA.
+// Roles (16 warps): 0-3 and 4-7 softmax of the two halves, 8-11 conversion, 12 and 14 product issue of the
+// halves, 13 TMA.
 #include "common.cuh"
 #include "gqa_fp8.cuh"
 #include "sm100.cuh"
@@ -32,13 +33,15 @@ constexpr int kThreads = 512;
 constexpr int kRows = 256;    // query rows of a problem
 constexpr int kTok = 128;     // tokens of a step
 constexpr int kStages = 4;    // raw ring: 64 tokens of K or V each
+constexpr int kParts = 4;     // a step's weights are handed over 32 tokens at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNoMax = -1e30f;
 // Registers: 512 threads x 128 = 2 x 128 x 184 (softmax) + 2 x 128 x 72 (the rest).
 constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
 
-// Scales of 16 tokens: ks * scale * log2 e, log2 vs, 1 / vs; ok: the tokens are there.
+// Scales of 16 tokens (equal over the tokens of a box): ks * scale * log2 e, log2 vs, 1 / vs; ok: 1 where the tokens are
+// there, 2 where all of the step's are.
 struct Scale {
   float kf, lsv, isv;
   int ok;
@@ -53,7 +56,6 @@ struct PrefillArgs {
   GqaArgs a;
   int32_t is_f16, group;
   int32_t least;   // query rows (rows x group) above which a lane is this kernel's
-  int32_t box;     // tokens of a TMA box: the largest of 16, 32, 64 that divides the page
   Rec* rec;        // [grid]
   float* part;     // [grid][2][256 * (D + 2)]
 };
@@ -69,32 +71,68 @@ struct Layout {
 
 // Control block, byte offsets.
 constexpr int kRawFull = 0, kRawEmpty = 32, kKFull = 64, kKEmpty = 80, kVFull = 96, kVEmpty = 112, kQFull = 128, kSFull = 144,
-              kPFull = 160, kOFull = 176, kDrain = 192, kSlot = 200, kAbort = 204, kScales = 256 /* [4][8] */,
-              kScan = 768 /* [16] */, kFound = 896 /* unit, lane */;
+              kPFull = 160 /* [half][part] */, kOFull = 224, kDrain = 240, kTurn = 256, kSlot = 272, kAbort = 276, kScales = 512 /* [4][8] */,
+              kScan = 1024 /* [16] */, kFound = 1152 /* step and lane, tile and its first step */;
 
 constexpr uint32_t idesc_f16(int n, int b_mn_major) {  // D fp32, A and B fp16, M = 128
   return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Products by one thread; descriptors as their low words (address, leading offset), which is all that changes.
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.b32 p, %5, 0;\nmov.b64 x, {%1, %3};\nmov.b64 y, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate));
 }
-__device__ __forceinline__ void umma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f16_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n.reg .pred p;\n.reg .b64 y;\nsetp.ne.b32 p, %5, 0;\nmov.b64 y, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate));
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
-      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+
+// 128 columns in one wait.
+__device__ __forceinline__ void tmem_ld128(uint32_t addr, float* v) {
+  uint32_t r[128];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%129];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(addr), "r"(addr + 64)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t d, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -107,6 +145,44 @@ __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32
   asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
       : "=r"(lo), "=r"(hi)
       : "r"(w));
+}
+
+// A wait of at most kTries tries (each of which may sleep for a while): short, as the kernel's code has to stay in the
+// instruction cache.  When it runs out it raises `abort`, which ends the others' waits.
+constexpr uint32_t kTries = 1u << 22;
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort, unsigned long long* err, unsigned site) {
+  uint32_t n = 0;
+  bool ok;
+#pragma unroll 1
+  while (!(ok = mbar_try_wait(bar, parity)) && !*abort && ++n < kTries) {
+  }
+  if (n == kTries) *abort = 1, hk_flag(err, hk::kErrWaitTimeout, site);
+  return ok;
+}
+
+// A warp's arrival: what its lanes did before is seen by who waits.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// 8 values of a row of Q (kLanes neighbouring lanes hold the row) scaled by a power of two, as fp16; *back undoes it.
+template <int kLanes>
+__device__ __noinline__ uint4 scaled_row(uint4 u, int is_f16, float* back) {
+  float f[8], top = 0.f;
+  if (is_f16) unpack8<true>(u, f);
+  else unpack8<false>(u, f);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+#pragma unroll
+  for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const int ex = (int)((__float_as_uint(top) >> 23) & 255);  // 0: zero or subnormal, 255: not finite
+  const int up = ex == 255 ? 0 : min(134 - ex, 120);
+  const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] *= mul;
+  *back = __uint_as_float((uint32_t)(127 - up) << 23);
+  return pack8<true>(f);
 }
 
 // A lane's rows of this kernel, 0 when it has none.
@@ -124,14 +200,33 @@ __device__ __forceinline__ Lane lane_at(const PrefillArgs& s, int b) {
   return x;
 }
 
-// Steps of one (row tile, head): up to the position of the tile's last row.
+// (Products of rows and heads fit 31 bits: Q itself takes 128 bytes or more for each.)
+__device__ __forceinline__ int tiles_of(const PrefillArgs& s, const Lane& x) { return (x.rows * s.group + kRows - 1) / kRows; }
+
+// Steps of one (row tile, head): up to the position of the tile's last row.  (Negative positions count as 0: their rows
+// see nothing.)
 __device__ __forceinline__ int steps_of(const PrefillArgs& s, const Lane& x, int tile) {
-  const int64_t upto = min((int64_t)x.rows, ((int64_t)(tile + 1) * kRows + s.group - 1) / s.group);
-  return (int)max((int64_t)1, (x.pos0 + upto + kTok - 1) / kTok);
+  const int upto = min(x.rows, (int)(((unsigned)(tile + 1) * kRows + s.group - 1) / (unsigned)s.group));
+  return (int)(((unsigned)max(x.pos0, 0) + upto + kTok - 1) / kTok);
 }
 
-__device__ __forceinline__ int tiles_of(const PrefillArgs& s, const Lane& x) {
-  return (int)(((int64_t)x.rows * s.group + kRows - 1) / kRows);
+// Steps of the first n tiles of a lane.  The last row of a tile but the lane's last is ceil(256 (tile + 1) / group) - 1, and
+// floor((floor(x / g) + b) / m) = floor((x + b g) / (m g)), so the steps are floors of a line: summed by the Euclidean
+// algorithm.
+__device__ __noinline__ int64_t steps_before(int group, int rows, int pos0, int n, int tiles) {
+  int64_t sum = 0;
+  if (n == tiles && n > 0) sum = ((int64_t)max(pos0, 0) + rows + kTok - 1) / kTok, --n;
+  int64_t count = n, m = (int64_t)kTok * group, step = kRows, at = kRows + group - 1 + ((int64_t)max(pos0, 0) + kTok - 1) * group;
+  while (count > 0) {
+    sum += (count - 1) * count / 2 * (step / m) + count * (at / m);
+    step %= m, at %= m;
+    const int64_t top = step * count + at;
+    if (top < m) break;
+    count = top / m, at = top % m;
+    const int64_t swap = m;
+    m = step, step = swap;
+  }
+  return sum;
 }
 
 // Walks a CTA's range of steps problem by problem.  Every role walks on its own.
@@ -165,7 +260,18 @@ struct Walk {
   }
 };
 
-template <int D>
+// Query row `at` of a lane as (token, head of the group), stepped without divisions.
+struct RowAt {
+  int t, h;
+  __device__ __forceinline__ RowAt(int at, int group) : t(at / group), h(at - at / group * group) {}
+  __device__ __forceinline__ void add(const RowAt& d, int group) {
+    t += d.t, h += d.h;
+    if (h >= group) h -= group, ++t;
+  }
+};
+
+// kBox: tokens that share a page for sure (16, 32 or 64), and so a pair of scales.
+template <int D, int kBox>
 __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s, const __grid_constant__ CUtensorMap kmap,
                                                                   const __grid_constant__ CUtensorMap vmap) {
   using L = Layout<D>;
@@ -182,14 +288,14 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
     return;
   }
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(bar(kRawFull, i), 1), mbar_init(bar(kRawEmpty, i), 128);
+    for (int i = 0; i < kStages; ++i) mbar_init(bar(kRawFull, i), 1), mbar_init(bar(kRawEmpty, i), 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kKFull, i), 128), mbar_init(bar(kKEmpty, i), 1);
-      mbar_init(bar(kVFull, i), 128), mbar_init(bar(kVEmpty, i), 1);
-      mbar_init(bar(kQFull, i), 128), mbar_init(bar(kSFull, i), 1);
-      mbar_init(bar(kPFull, i), 128), mbar_init(bar(kOFull, i), 1);
+      mbar_init(bar(kKFull, i), 4), mbar_init(bar(kKEmpty, i), 2);  // (empty: both halves' products)
+      mbar_init(bar(kVFull, i), 4), mbar_init(bar(kVEmpty, i), 2);
+      mbar_init(bar(kDrain, i), 1), mbar_init(bar(kTurn, i), 4);
+      mbar_init(bar(kQFull, i), 4), mbar_init(bar(kSFull, i), 1), mbar_init(bar(kOFull, i), 1);
+      for (int k = 0; k < kParts; ++k) mbar_init(bar(kPFull, kParts * i + k), 4);
     }
-    mbar_init(bar(kDrain), 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -203,8 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
     if (b < a.num_lanes) {
       if (blockIdx.x == 0 && a.cu[b + 1] - a.cu[b] > a.max_rows) hk_flag(a.err, hk::kErrLaneRows, (unsigned)b);
       const Lane x = lane_at(s, b);
-      if (x.rows)
-        for (int i = 0, m = tiles_of(s, x); i < m; ++i) n += steps_of(s, x, i);
+      if (x.rows) n = steps_before(s.group, x.rows, x.pos0, tiles_of(s, x), tiles_of(s, x));
     }
     return n * a.kv_heads;
   };
@@ -253,16 +358,19 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
   Walk w;
   w.u = 0, w.end = (int)(u1 - u0), w.steps = 1, w.tiles = 0, w.tile = 0, w.lane = 0, w.begin = 0;
   if (u0 < u1) {
-    int64_t at = found[0] - u0;  // where the lane begins, at or before the range
     w.lane = (int)found[1];
     w.x = lane_at(s, w.lane);
     w.tiles = tiles_of(s, w.x);
-    w.steps = steps_of(s, w.x, 0);
-    while (at + (int64_t)w.steps * a.kv_heads <= 0) {  // the tile in which the range begins
-      at += (int64_t)w.steps * a.kv_heads;
-      w.steps = steps_of(s, w.x, ++w.tile);
+    // The tile in which the range begins: every thread tries its own.
+    const int64_t into = u0 - found[0];
+    for (int i = tid; i < w.tiles; i += kThreads) {
+      const int64_t from = steps_before(s.group, w.x.rows, w.x.pos0, i, w.tiles) * a.kv_heads;
+      if (from <= into && into < from + (int64_t)steps_of(s, w.x, i) * a.kv_heads) found[2] = i, found[3] = from - into;
     }
-    w.begin = (int)at;
+    __syncthreads();
+    w.tile = (int)found[2];
+    w.begin = (int)found[3];
+    w.steps = steps_of(s, w.x, w.tile);
   }
   Scale* scales = reinterpret_cast<Scale*>(ctl + kScales);
 
@@ -272,8 +380,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lanes + half * 128, o_col = tmem + lanes + 256 + half * 128;
-    uint8_t* q_row = smem + L::kQ + half * L::kTile + row * 128;
-    uint32_t n_s = 0, n_o = 0, step = 0;
+    uint8_t* q_rows = smem + L::kQ + half * L::kTile + (warp & 3) * 32 * 128;  // of this warp
+    uint32_t n_s = 0, n_o = 0, n_turn = 0, step = 0;
     bool live = true;
     while (live && w.next(s)) {
       if (w.rows_left <= half * 128) {  // no rows for this half
@@ -281,80 +389,92 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
         continue;
       }
       const int r = half * 128 + row;
+      const bool both = w.rows_left > 128;
       const bool on = r < w.rows_left;
-      const int at = w.row0 + r, t = w.x.t0 + (on ? at / s.group : 0);
-      const int64_t y = (int64_t)t * a.q_heads + w.g * s.group + (on ? at - at / s.group * s.group : 0);
-      const int pos = on ? a.positions[t] : INT32_MAX;
-      float rowf;
-      {  // this row of Q, scaled by a power of two so that fp16 holds it exactly
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + t * a.q_stride + (y - (int64_t)t * a.q_heads) * D);
-        float top = 0.f;
-#pragma unroll 4
-        for (int i = 0; i < D / 8; ++i) {
-          float f[8];
-          const uint4 u = on ? src[i] : make_uint4(0, 0, 0, 0);
-          if (s.is_f16) unpack8<true>(u, f);
-          else unpack8<false>(u, f);
+      const int pos = on ? a.positions[w.x.t0 + (w.row0 + r) / s.group] : INT32_MAX;
+      float rowf = 1.f;
+      // This warp's 32 rows of Q, D / 8 lanes to a row; each row scaled by a power of two so that fp16 holds it exactly.
+      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kBatch = 8;
+      const int part = lane % kLanes;
+      RowAt q_at(w.row0 + r - lane + lane / kLanes, s.group);
+      const RowAt q_step(kAtOnce, s.group);
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
+        uint4 u[kBatch];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+        for (int i = 0; i < kBatch; ++i) {
+          u[i] = make_uint4(0, 0, 0, 0);
+          if (r - lane + (i0 + i) * kAtOnce + lane / kLanes < w.rows_left)
+            u[i] = *reinterpret_cast<const uint4*>(a.q + (w.x.t0 + q_at.t) * a.q_stride + (int64_t)(w.g * s.group + q_at.h) * D + part * 8);
+          q_at.add(q_step, s.group);
         }
-        const int ex = (int)((__float_as_uint(top) >> 23) & 255);
-        const int up = ex == 255 ? 0 : min(134 - ex, 120);
-        const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-        rowf = __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll 4
-        for (int i = 0; i < D / 8; ++i) {
-          float f[8];
-          const uint4 u = on ? src[i] : make_uint4(0, 0, 0, 0);
-          if (s.is_f16) unpack8<true>(u, f);
-          else unpack8<false>(u, f);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= mul;
-          *reinterpret_cast<uint4*>(q_row + (i >> 3) * L::kHalf + (((i & 7) ^ (row & 7)) << 4)) = pack8<true>(f);
+        for (int i = 0; i < kBatch; ++i) {
+          const int wr = (i0 + i) * kAtOnce + lane / kLanes;  // row of the warp
+          float mine;
+          const uint4 x = scaled_row<kLanes>(u[i], s.is_f16, &mine);
+          *reinterpret_cast<uint4*>(q_rows + (part >> 3) * L::kHalf + wr * 128 + (((part & 7) ^ (wr & 7)) << 4)) = x;
+          const float back = __shfl_sync(0xffffffffu, mine, lane % kAtOnce * kLanes);
+          if (lane / kAtOnce == i0 + i) rowf = back;
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(bar(kQFull, half));
+      warp_arrive(bar(kQFull, half));
       // The smallest position of this half: rows of a lane rise.
       const int pos_min = w.x.pos0 + (w.row0 + half * 128) / s.group;
 
       float m = kNoMax, l = 0.f;
       for (int i = w.first; i < w.last; ++i, ++n_s, ++step) {
-        live = live && mbar_wait(bar(kSFull, half), n_s & 1, abort, a.err, 0x70);
+        live = live && wait_bar(bar(kSFull, half), n_s & 1, abort, a.err, 0x70);
         live = __all_sync(0xffffffffu, live);
         if (!live) break;
+        // The halves take turns: while one half's weights are computed, the other half's products run.
+        if (both) {
+          live = wait_bar(bar(kTurn, half), (n_turn & 1) ^ (half ^ 1), abort, a.err, 0x79);
+          live = __all_sync(0xffffffffu, live);
+          if (!live) break;
+          ++n_turn;
+        }
         tc_fence_after();
         float v[128];
-        tmem_ld64(s_col, v);
-        tmem_ld64(s_col + 64, v + 64);
+        tmem_ld128(s_col, v);
+        constexpr int kGroups = kTok / kBox;
         const Scale* sc = scales + (step & 3) * 8;
-        const bool edge = (i + 1) * kTok - 1 > pos_min;
-        float top = -INFINITY;
-        if (!edge) {
+        // Few groups keep their scales in registers; many read them again (shared memory) for each of the two passes.
+        constexpr bool kKeep = kGroups <= 2;
+        float f_kept[2] = {1.f, 1.f}, lsv_kept[2] = {0.f, 0.f};
+        if (kKeep) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float x = v[16 * k];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) x = fmaxf(x, v[16 * k + e]);
-            top = fmaxf(top, fmaf(x, sc[k].kf * rowf, sc[k].lsv));  // the factor is positive
-          }
-        } else {
+          for (int k = 0; k < 2; ++k) f_kept[k] = fmaxf(sc[4 * k].kf * rowf, 1.1754944e-38f), lsv_kept[k] = sc[4 * k].lsv;
+        }
+        auto factor = [&](int k) { return kKeep ? f_kept[k & 1] : fmaxf(sc[k * (kBox / 16)].kf * rowf, 1.1754944e-38f); };  // above 0: a masked -inf stays one
+        auto addend = [&](int k) { return kKeep ? lsv_kept[k & 1] : sc[k * (kBox / 16)].lsv; };
+        if ((i + 1) * kTok - 1 > pos_min) {
           const int seen = pos - i * kTok;  // tokens after it are masked
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
+          for (int e = 0; e < 128; ++e) v[e] = e > seen ? -INFINITY : v[e];
+        }
+        float top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = fmaf(v[16 * k + e], sc[k].kf * rowf, sc[k].lsv);
-              v[16 * k + e] = 16 * k + e > seen ? -INFINITY : x;
-              top = fmaxf(top, v[16 * k + e]);
-            }
+        for (int k = 0; k < kGroups; ++k) {
+          float x[4];  // chains
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = max3(v[kBox * k + e], v[kBox * k + 4 + e], v[kBox * k + 8 + e]);
+#pragma unroll
+          for (int e = 12; e < kBox - 4; e += 8)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[y] = max3(x[y], v[kBox * k + e + y], v[kBox * k + e + 4 + y]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = fmaxf(x[e], v[kBox * k + kBox - 4 + e]);
+          const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          top = fmaxf(top, fmaf(most, factor(k), addend(k)));  // the factor is positive
         }
         // S is complete, so the product before it (which this row's O is from) is too.
         const bool over = top > m + 8.f;
         if (__any_sync(0xffffffffu, over)) {
-          const float m_new = over ? top : m, f = exp2_approx(m - m_new);
+          const float m_new = over ? top : m, down = exp2_approx(m - m_new);
           m = m_new;
-          l *= f;
+          l *= down;
           if (i > w.first) {
 #pragma unroll 1
             for (int k = 0; k < D / 16; ++k) {
@@ -362,67 +482,84 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
               tmem_ld16(o_col + 16 * k, o);
               uint32_t x[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * f);
-              asm volatile(
-                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(o_col + 16 * k),
-                  "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]),
-                  "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
-                  : "memory");
+              for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * down);
+              tmem_st16(o_col + 16 * k, x);
             }
           }
         }
-        uint32_t p[32];  // 64 tokens' weights at a time, over columns of S that are read already
+        // 32 tokens' weights at a time, over columns of S that are read already: their product starts while the others are
+        // weighed.
+        uint64_t sum = 0;  // two zeros
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float f = edge ? 1.f : sc[k].kf * rowf, c = (edge ? 0.f : sc[k].lsv) - m;
-          float sum = 0.f;
+        for (int j = 0; j < kParts; ++j) {
+          uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float x0 = exp2_approx(fmaf(v[16 * k + e], f, c)), x1 = exp2_approx(fmaf(v[16 * k + e + 1], f, c));
-            sum += x0 + x1;
-            p[8 * (k & 3) + e / 2] = pack2<true>(x0, x1);
+          for (int e = 0; e < 32; e += 2) {
+            const int t = 32 * j + e, k = t / kBox;
+            const float f = factor(k), c = addend(k) - m;
+            float x0, x1;
+            unpair(fma2(pair(v[t], v[t + 1]), pair(f, f), pair(c, c)), x0, x1);
+            x0 = exp2_approx(x0), x1 = exp2_approx(x1);
+            sum = add2(sum, pair(x0, x1));
+            p[e / 2] = pack2<true>(x0, x1);
+            if ((t + 2) % kBox == 0) {
+              float s0, s1;
+              unpair(sum, s0, s1);
+              l = fmaf(s0 + s1, sc[k * (kBox / 16)].isv, l);
+              sum = 0;
+            }
           }
-          l = fmaf(sum, sc[k].isv, l);
-          if ((k & 3) == 3) tmem_st32(s_col + 8 * (k - 3), p);
+          tmem_st16(s_col + 16 * j, p);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
+          warp_arrive(bar(kPFull, half * kParts + j));
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tc_fence_before();
-        mbar_arrive(bar(kPFull, half));
+        if (both) warp_arrive(bar(kTurn, half ^ 1));
       }
-      live = live && mbar_wait(bar(kOFull, half), n_o & 1, abort, a.err, 0x71);
+      live = live && wait_bar(bar(kOFull, half), n_o & 1, abort, a.err, 0x71);
       live = __all_sync(0xffffffffu, live);
       if (!live) break;
       ++n_o;
       tc_fence_after();
-      const bool starts = w.first == 0;
-      if (starts && w.last == w.steps) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+      // O leaves by way of this warp's rows of Q (both products are done with them), so that a row is written by
+      // neighbouring lanes: 32 dims at a time, as fp32 in a 128-byte line for each row, 16-byte parts swizzled.
+      const bool starts = w.first == 0, whole = starts && w.last == w.steps;
+      float* piece = s.part + ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (kRows * (D + 2));
+      const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      const RowAt out_step(4, s.group);
+      const RowAt out_first(w.row0 + r - lane + lane / 8, s.group);
+#pragma unroll 1
+      for (int k = 0; k < D / 32; ++k) {  // 32 dims: 128 bytes a row
+        float o[32];
+        tmem_ld32(o_col + 32 * k, o);
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          float o[32];
-          tmem_ld32(o_col + 32 * k, o);
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<float4*>(q_rows + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+              make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
+        __syncwarp();
+        RowAt at = out_first;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= inv;
-          if (on) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              *reinterpret_cast<uint4*>(a.out + y * D + 32 * k + e) = s.is_f16 ? pack8<true>(o + e) : pack8<false>(o + e);
+        for (int i = 0; i < 8; ++i) {  // 4 rows at once, 8 lanes each
+          const int wr = i * 4 + lane / 8, qr = r - lane + wr;
+          const float4 x = *reinterpret_cast<const float4*>(q_rows + wr * 128 + (((lane & 7) ^ (wr & 7)) << 4));
+          if (qr < w.rows_left) {
+            if (whole) {
+              const int64_t y = (int64_t)(w.x.t0 + at.t) * a.q_heads + w.g * s.group + at.h;
+              *reinterpret_cast<uint2*>(a.out + y * D + 32 * k + (lane & 7) * 4) =
+                  s.is_f16 ? make_uint2(pack2<true>(x.x, x.y), pack2<true>(x.z, x.w)) : make_uint2(pack2<false>(x.x, x.y), pack2<false>(x.z, x.w));
+            } else {
+              *reinterpret_cast<float4*>(piece + qr * D + 32 * k + (lane & 7) * 4) = x;
+            }
           }
+          at.add(out_step, s.group);
         }
-        if (on) a.lse[y] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
-      } else {
-        float* part = s.part + ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (kRows * (D + 2));
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          float o[32];
-          tmem_ld32(o_col + 32 * k, o);
-          if (on) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(part + r * D + 32 * k + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-        }
-        if (on) part[kRows * D + r] = m, part[kRows * (D + 1) + r] = l;
+        __syncwarp();
+      }
+      if (on && whole) {
+        const int at = w.row0 + r, t = at / s.group;
+        a.lse[(int64_t)(w.x.t0 + t) * a.q_heads + w.g * s.group + at - t * s.group] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
+      } else if (on) {
+        piece[kRows * D + r] = m, piece[kRows * (D + 1) + r] = l;
       }
       tc_fence_before();
     }
@@ -431,7 +568,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
     if (warp < 12) {
       // ---- conversion: raw e4m3 -> swizzled fp16 -----------------------------------------------
       const int id = tid - 256;
-      constexpr int kPer = 64 * D / 16 / 128;  // 16-byte parts of a stage a thread converts
+      constexpr int kPer = 64 * D / 16 / 128;  // 16-byte parts of a stage a thread converts: id, id + 128, ...
+      // Part id: its place in the raw lines, its token and dims, and its two places in the fp16 tile (the second 64 dims are
+      // written in the other order: the two halves of a row share banks).  The next parts lie at fixed distances.
+      const int src = (id >> 3) * 128 + (((id & 7) ^ (id >> 3 & 7)) << 4);
+      const int t0 = id / (D / 16), p0 = id % (D / 16), c0 = 2 * (p0 & 3);
+      const bool second = p0 >= 4;
+      const int dst = (p0 >> 2) * L::kHalf + t0 * 128, dst_first = dst + (((c0 + second) ^ (t0 & 7)) << 4), dst_other = dst + (((c0 + !second) ^ (t0 & 7)) << 4);
       uint32_t n = 0, step = 0;                // stages read
       bool live = true;
       while (live && w.next(s)) {
@@ -440,103 +583,112 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
           const Scale* sc = scales + (step & 3) * 8;
 #pragma unroll 1
           for (int kv = 0; kv < 2 && live; ++kv) {
-            live = mbar_wait(bar(kv ? kVEmpty : kKEmpty, step & 1), (step >> 1 & 1) ^ 1, abort, a.err, 0x72);
+            live = __all_sync(0xffffffffu, wait_bar(bar(kv ? kVEmpty : kKEmpty, step & 1), (step >> 1 & 1) ^ 1, abort, a.err, 0x72));
             uint8_t* tile = smem + (kv ? L::kV : L::kK) + (step & 1) * L::kTile;
 #pragma unroll 1
             for (int h = 0; h < 2 && live; ++h, ++n) {
               const int stage = n % kStages;
-              live = mbar_wait(bar(kRawFull, stage), n / kStages & 1, abort, a.err, 0x73);
+              live = live && __all_sync(0xffffffffu, wait_bar(bar(kRawFull, stage), n / kStages & 1, abort, a.err, 0x73));
               if (!live) break;
-              const uint8_t* raw = smem + L::kRing + stage * L::kRaw;
+              const uint8_t* raw = smem + L::kRing + stage * L::kRaw + src;
               uint4 u[kPer];
 #pragma unroll
-              for (int k = 0; k < kPer; ++k) {
-                const int part = id + 128 * k, t = part / (D / 16), line = part >> 3;
-                const bool ok = sc[h * 4 + t / 16].ok && i * kTok + h * 64 + t < len;
-                u[k] = ok ? *reinterpret_cast<const uint4*>(raw + line * 128 + (((part & 7) ^ (line & 7)) << 4)) : make_uint4(0, 0, 0, 0);
+              for (int k = 0; k < kPer; ++k) u[k] = *reinterpret_cast<const uint4*>(raw + k * 2048);
+              if (sc[0].ok != 2) {  // some tokens are not there, or past the lane's end
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                  const int t = h * 64 + t0 + k * (128 * 16 / D);
+                  if (!sc[t / 16].ok || i * kTok + t >= len) u[k] = make_uint4(0, 0, 0, 0);
+                }
               }
-              mbar_arrive(bar(kRawEmpty, stage));
+              warp_arrive(bar(kRawEmpty, stage));
+              uint8_t* to = tile + h * (64 * 128);
 #pragma unroll
               for (int k = 0; k < kPer; ++k) {
-                const int part = id + 128 * k, t = h * 64 + part / (D / 16), p = part % (D / 16);
                 uint4 lo, hi;
                 e4m3x4_to_f16x4(u[k].x, lo.x, lo.y), e4m3x4_to_f16x4(u[k].y, lo.z, lo.w);
                 e4m3x4_to_f16x4(u[k].z, hi.x, hi.y), e4m3x4_to_f16x4(u[k].w, hi.z, hi.w);
-                uint8_t* dst = tile + (p >> 2) * L::kHalf + t * 128;
-                const int c = 2 * (p & 3), x = t & 7;
-                // The second 64 dims in the other order: the two halves of a row share banks.
-                const bool second = p >= 4;
-                *reinterpret_cast<uint4*>(dst + (((c + second) ^ x) << 4)) = second ? hi : lo;
-                *reinterpret_cast<uint4*>(dst + (((c + !second) ^ x) << 4)) = second ? lo : hi;
+                *reinterpret_cast<uint4*>(to + dst_first + k * (128 * 16 / D * 128)) = second ? hi : lo;
+                *reinterpret_cast<uint4*>(to + dst_other + k * (128 * 16 / D * 128)) = second ? lo : hi;
               }
             }
             if (!live) break;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(bar(kv ? kVFull : kKFull, step & 1));
+            warp_arrive(bar(kv ? kVFull : kKFull, step & 1));
           }
         }
       }
-    } else if (warp == 12) {
-      // ---- product issue ----------------------------------------------------------------------
+    } else if (warp == 12 || warp == 14) {
+      // ---- product issue: a warp for each half, so that neither waits for the other's weights ---------
+      const int h = (warp - 12) / 2;
       if (lane == 0) {
-        const uint64_t q_desc = sdesc_sw128(base + L::kQ, 16, 1024), k_desc = sdesc_sw128(base + L::kK, 16, 1024),
-                       v_desc = sdesc_sw128(base + L::kV, L::kHalf, 1024);
-        uint32_t step = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
+        const uint64_t desc = sdesc_sw128(base, 16, 1024);
+        const uint32_t hi = (uint32_t)(desc >> 32), q = (uint32_t)desc + ((L::kQ + h * L::kTile) >> 4), k0 = (uint32_t)desc + (L::kK >> 4);
+        const uint32_t v0 = (uint32_t)sdesc_sw128(base + L::kV, L::kHalf, 1024);
+        const uint32_t s_at = tmem + h * 128, o_at = tmem + 256 + h * 128;
+        uint32_t step = 0, n_q = 0, n_p = 0;
         bool live = true;
-        auto scores = [&](int h, uint32_t st) {
+        auto scores = [&](uint32_t st) {
+          const uint32_t k = k0 + ((st & 1) ? (uint32_t)(L::kTile >> 4) : 0u);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = ((k >> 2) * L::kHalf + (k & 3) * 32) >> 4;
-            umma_f16(tmem + h * 128, q_desc + (h * L::kTile >> 4) + off, k_desc + ((st & 1) * L::kTile >> 4) + off, idesc_f16(kTok, 0), k != 0);
+          for (int i = 0; i < D / 16; ++i) {
+            const uint32_t off = ((i >> 2) * L::kHalf + (i & 3) * 32) >> 4;
+            umma_f16(s_at, q + off, k + off, hi, idesc_f16(kTok, 0), i != 0);
           }
           umma_commit(bar(kSFull, h));
+          umma_commit(bar(kKEmpty, st & 1));
         };
+        auto full = [&](int which, uint32_t st) { return wait_bar(bar(which, st & 1), st >> 1 & 1, abort, a.err, 0x74); };
         while (live && w.next(s)) {
-          const int halves = w.rows_left > 128 ? 2 : 1, n = w.last - w.first;
-          live = live && mbar_wait(bar(kKFull, step & 1), step >> 1 & 1, abort, a.err, 0x74);
-          for (int h = 0; h < halves && live; ++h) {
-            live = mbar_wait(bar(kQFull, h), n_q[h]++ & 1, abort, a.err, 0x75);
-            if (!live) break;
-            tc_fence_after();
-            scores(h, step);
+          const int n = w.last - w.first;
+          if (w.rows_left <= h * 128) {  // no rows for this half: its share of the buffers is free as soon as they are full
+            for (int i = 0; i < n && live; ++i, ++step) {
+              live = full(kKFull, step);
+              if (live) mbar_arrive(bar(kKEmpty, step & 1));
+              live = live && full(kVFull, step);
+              if (live) mbar_arrive(bar(kVEmpty, step & 1));
+            }
+            continue;
           }
-          if (live) umma_commit(bar(kKEmpty, step & 1));
-          for (int i = 0; i < n && live; ++i, ++step) {
-            live = mbar_wait(bar(kVFull, step & 1), step >> 1 & 1, abort, a.err, 0x76);
-            const bool more = i + 1 < n;
-            for (int h = 0; h < halves && live; ++h) {
-              live = mbar_wait(bar(kPFull, h), n_p[h]++ & 1, abort, a.err, 0x77);
+          live = full(kKFull, step) && wait_bar(bar(kQFull, h), n_q++ & 1, abort, a.err, 0x75);
+          if (!live) break;
+          tc_fence_after();
+          scores(step);
+          for (int i = 0; i < n && live; ++i, ++step, ++n_p) {
+            const uint32_t v = v0 + ((step & 1) ? (uint32_t)(L::kTile >> 4) : 0u);
+            live = full(kVFull, step);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              live = live && wait_bar(bar(kPFull, h * kParts + part), n_p & 1, abort, a.err, 0x77);
               if (!live) break;
               tc_fence_after();
 #pragma unroll
-              for (int k = 0; k < kTok / 16; ++k)
-                umma_f16_tmem(tmem + 256 + h * 128, tmem + h * 128 + k * 8, v_desc + (((step & 1) * L::kTile + k * 2048) >> 4), idesc_f16(D, 1),
-                              i > 0 || k > 0);
-              if (more) {
-                if (h == 0) live = mbar_wait(bar(kKFull, (step + 1) & 1), (step + 1) >> 1 & 1, abort, a.err, 0x74);
-                if (!live) break;
-                scores(h, step + 1);
-              } else {
-                umma_commit(bar(kOFull, h));
-              }
+              for (int k = 2 * part; k < 2 * part + 2; ++k)
+                umma_f16_tmem(o_at, s_at + k * 8, v + (k * 2048 >> 4), hi, idesc_f16(D, 1), k > 0 ? 1u : (uint32_t)(i > 0));
             }
             if (!live) break;
             umma_commit(bar(kVEmpty, step & 1));
-            if (more) umma_commit(bar(kKEmpty, (step + 1) & 1));
+            if (i + 1 < n) {
+              live = full(kKFull, step + 1);
+              if (!live) break;
+              tc_fence_after();
+              scores(step + 1);
+            } else {
+              umma_commit(bar(kOFull, h));
+            }
           }
         }
         // Every product issued is complete before tensor memory is freed.
-        umma_commit(bar(kDrain));
-        *abort = *abort || !live;
+        umma_commit(bar(kDrain, h));
         const unsigned long long t0 = globaltimer();
-        while (!mbar_try_wait(bar(kDrain), 0) && globaltimer() - t0 < 1000000000ull) {
+        while (!mbar_try_wait(bar(kDrain, h), 0) && globaltimer() - t0 < 1000000000ull) {
         }
       }
     } else if (warp == 13) {
       // ---- TMA: lanes 0-7 hold 16 tokens of the step each -----------------------------------------
       uint32_t n = 0, step = 0;
       bool live = true;
-      const int boxes = s.box / 16;
+      constexpr int boxes = kBox / 16;
       Rec rec = {-1, 0, 0, 0};
       while (live && w.next(s)) {
         if (w.first == 0 && w.last < w.steps) rec.lane = w.lane, rec.g = w.g, rec.row0 = w.row0;
@@ -561,18 +713,20 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
           if (page == -2) hk_flag(a.err, hk::kErrAttnPage, (unsigned)w.lane);
           int32_t line = 0;
           if (page >= 0) line = (int32_t)((((int64_t)page * a.kv_heads + w.g) * a.page_size + (i * kTok + 16 * lane) % a.page_size) * D / 128);
-          const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && lane % boxes == 0);
+          const unsigned pages = __ballot_sync(0xffffffffu, page >= 0);
+          const unsigned there = pages & (boxes == 1 ? 0xffu : boxes == 2 ? 0x55u : 0x11u);
+          const int ok = pages == 0xffu && (i + 1) * kTok <= len ? 2 : 1;
           vs = fmaxf(vs, 7.8886090522101181e-31f);
 #pragma unroll 1
           for (int part = 0; part < 4 && live; ++part, ++n) {  // K, K, V, V: 64 tokens each
             const int stage = n % kStages, h = part & 1;
-            live = mbar_wait(bar(kRawEmpty, stage), (n / kStages & 1) ^ 1, abort, a.err, 0x78);
+            live = wait_bar(bar(kRawEmpty, stage), (n / kStages & 1) ^ 1, abort, a.err, 0x78);
             live = __all_sync(0xffffffffu, live);
             if (!live) break;
             // The step's scales: their place was last read four steps ago, before the products that freed this stage.
-            if (part == 0 && lane < 8) scales[(step & 3) * 8 + lane] = page >= 0 ? Scale{ks * (a.scale * kLog2e), log2f(vs), 1.f / vs, 1} : Scale{1.f, -INFINITY, 0.f, 0};
+            if (part == 0 && lane < 8) scales[(step & 3) * 8 + lane] = page >= 0 ? Scale{ks * (a.scale * kLog2e), log2f(vs), 1.f / vs, ok} : Scale{1.f, -INFINITY, 0.f, 0};
             __syncwarp();
-            if (lane == 0) mbar_expect_tx(bar(kRawFull, stage), (uint32_t)__popc(there & (0xfu << (4 * h))) * s.box * D);
+            if (lane == 0) mbar_expect_tx(bar(kRawFull, stage), (uint32_t)__popc(there & (0xfu << (4 * h))) * (kBox * D));
             __syncwarp();
             if ((there >> lane & 1) && lane / 4 == h)
               tma_load_2d(base + L::kRing + stage * L::kRaw + (lane & 3) * 16 * D, part < 2 ? &kmap : &vmap, bar(kRawFull, stage), 0, line);
@@ -619,7 +773,7 @@ __global__ void __launch_bounds__(256) gqa_prefill_merge_kernel(PrefillArgs s, i
   if (lane == 0) a.lse[y] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
 }
 
-template <int D>
+template <int D, int kBox>
 int launch(PrefillArgs& s, int64_t steps, cudaStream_t stream) {
   using L = Layout<D>;
   static_assert(L::kBytes <= 232448, "shared memory");
@@ -628,16 +782,24 @@ int launch(PrefillArgs& s, int64_t steps, cudaStream_t stream) {
   const uint64_t lines = (uint64_t)s.a.num_pages * s.a.kv_heads * s.a.page_size * D / 128;
   HK_REQUIRE(lines <= INT32_MAX, "the cache's K and V arrays must be below 2^38 bytes each");
   CUtensorMap kmap, vmap;
-  HK_TRY(make_map_u8(&kmap, s.a.kc, lines, 128, s.box * D / 128));
-  HK_TRY(make_map_u8(&vmap, s.a.vc, lines, 128, s.box * D / 128));
-  HK_TRY_CUDA(cudaFuncSetAttribute(gqa_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
-  gqa_prefill_kernel<D><<<grid, kThreads, L::kBytes, stream>>>(s, kmap, vmap);
+  HK_TRY(make_map_u8(&kmap, s.a.kc, lines, 128, kBox * D / 128));
+  HK_TRY(make_map_u8(&vmap, s.a.vc, lines, 128, kBox * D / 128));
+  HK_TRY_CUDA(cudaFuncSetAttribute(gqa_prefill_kernel<D, kBox>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  gqa_prefill_kernel<D, kBox><<<grid, kThreads, L::kBytes, stream>>>(s, kmap, vmap);
   HK_TRY_LAUNCH("gqa_prefill_kernel");
   if (grid > 1) {
     gqa_prefill_merge_kernel<D><<<dim3(grid, kRows / 8), 256, 0, stream>>>(s, grid);
     HK_TRY_LAUNCH("gqa_prefill_merge_kernel");
   }
   return HK_OK;
+}
+
+template <int D>
+int launch(PrefillArgs& s, int64_t steps, cudaStream_t stream) {
+  // The largest box of 16, 32 or 64 tokens that divides the page.
+  if (s.a.page_size % 64 == 0) return launch<D, 64>(s, steps, stream);
+  if (s.a.page_size % 32 == 0) return launch<D, 32>(s, steps, stream);
+  return launch<D, 16>(s, steps, stream);
 }
 
 }  // namespace
@@ -656,7 +818,6 @@ int gqa_prefill(const GqaArgs& a, int32_t dtype, int32_t least, int64_t max_kv_l
   s.is_f16 = dtype == HK_F16;
   s.group = a.q_heads / a.kv_heads;
   s.least = least;
-  s.box = a.page_size % 64 == 0 ? 64 : a.page_size % 32 == 0 ? 32 : 16;
   s.rec = (Rec*)workspace;
   s.part = (float*)((uint8_t*)workspace + (size_t)sm_count() * sizeof(Rec));
   // At most this many steps: each lane's last row tile may be partly filled.
