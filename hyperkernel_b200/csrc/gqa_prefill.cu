@@ -33,6 +33,7 @@ constexpr int kThreads = 512;
 constexpr int kRows = 256;    // query rows of a problem
 constexpr int kTok = 128;     // tokens of a step
 constexpr int kStages = 4;    // raw ring: 64 tokens of K or V each
+constexpr int kStart = 2;     // what a problem costs besides its steps, in steps
 constexpr int kParts = 4;     // a step's weights are handed over 32 tokens at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -168,7 +169,7 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
 
 // 8 values of a row of Q (kLanes neighbouring lanes hold the row) scaled by a power of two, as fp16; *back undoes it.
 template <int kLanes>
-__device__ __noinline__ uint4 scaled_row(uint4 u, int is_f16, float* back) {
+__device__ __forceinline__ uint4 scaled_row(uint4 u, int is_f16, float* back) {
   float f[8], top = 0.f;
   if (is_f16) unpack8<true>(u, f);
   else unpack8<false>(u, f);
@@ -210,12 +211,12 @@ __device__ __forceinline__ int steps_of(const PrefillArgs& s, const Lane& x, int
   return (int)(((unsigned)max(x.pos0, 0) + upto + kTok - 1) / kTok);
 }
 
-// Steps of the first n tiles of a lane.  The last row of a tile but the lane's last is ceil(256 (tile + 1) / group) - 1, and
+// Units (steps and starts) of the first n tiles of a lane.  The last row of a tile but the lane's last is ceil(256 (tile + 1) / group) - 1, and
 // floor((floor(x / g) + b) / m) = floor((x + b g) / (m g)), so the steps are floors of a line: summed by the Euclidean
 // algorithm.
-__device__ __noinline__ int64_t steps_before(int group, int rows, int pos0, int n, int tiles) {
-  int64_t sum = 0;
-  if (n == tiles && n > 0) sum = ((int64_t)max(pos0, 0) + rows + kTok - 1) / kTok, --n;
+__device__ __noinline__ int64_t units_before(int group, int rows, int pos0, int n, int tiles) {
+  int64_t sum = (int64_t)n * kStart;
+  if (n == tiles && n > 0) sum += ((int64_t)max(pos0, 0) + rows + kTok - 1) / kTok, --n;
   int64_t count = n, m = (int64_t)kTok * group, step = kRows, at = kRows + group - 1 + ((int64_t)max(pos0, 0) + kTok - 1) * group;
   while (count > 0) {
     sum += (count - 1) * count / 2 * (step / m) + count * (at / m);
@@ -229,33 +230,36 @@ __device__ __noinline__ int64_t steps_before(int group, int rows, int pos0, int 
   return sum;
 }
 
-// Walks a CTA's range of steps problem by problem.  Every role walks on its own.
+// Walks a CTA's range problem by problem.  Every role walks on its own.  A problem counts kStart units for its beginning and
+// end (Q, the pipeline's filling, the output) before its steps.
 struct Walk {
-  int u, end;           // next step and end of the range, from its start
-  int begin;            // step at which the current tile begins (its heads follow one another)
+  int u, end;           // next unit and end of the range, from its start
+  int begin;            // unit at which the current tile begins (its heads follow one another)
   int lane, tile, tiles, steps;
   Lane x;
-  // The current problem.
+  // The current problem, and its steps in this range.
   int g, row0, first, last, rows_left;
 
   __device__ __forceinline__ bool next(const PrefillArgs& s) {
-    if (u >= end) return false;
-    while (u - begin >= steps * s.a.kv_heads) {
-      begin += steps * s.a.kv_heads;
-      if (++tile >= tiles) {
-        do {
-          x = lane_at(s, ++lane);
-        } while (x.rows == 0);
-        tile = 0, tiles = tiles_of(s, x);
+    do {
+      if (u >= end) return false;
+      while (u - begin >= (steps + kStart) * s.a.kv_heads) {
+        begin += (steps + kStart) * s.a.kv_heads;
+        if (++tile >= tiles) {
+          do {
+            x = lane_at(s, ++lane);
+          } while (x.rows == 0);
+          tile = 0, tiles = tiles_of(s, x);
+        }
+        steps = steps_of(s, x, tile);
       }
-      steps = steps_of(s, x, tile);
-    }
-    g = (u - begin) / steps;
-    first = u - begin - g * steps;
-    last = min(steps, first + (end - u));
+      g = (u - begin) / (steps + kStart);
+      const int lo = u - begin - g * (steps + kStart), hi = min(steps + kStart, lo + (end - u));
+      first = max(0, lo - kStart), last = max(0, hi - kStart);
+      u += hi - lo;
+    } while (first == last);  // the range ends before the problem's first step
     row0 = tile * kRows;
     rows_left = x.rows * s.group - row0;
-    u += last - first;
     return true;
   }
 };
@@ -304,12 +308,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
   // This CTA's range of steps, and the lane in which it begins.
   int64_t* scan = reinterpret_cast<int64_t*>(ctl + kScan);
   int64_t* found = reinterpret_cast<int64_t*>(ctl + kFound);
-  auto lane_steps = [&](int b) {
+  auto lane_units = [&](int b) {
     int64_t n = 0;
     if (b < a.num_lanes) {
       if (blockIdx.x == 0 && a.cu[b + 1] - a.cu[b] > a.max_rows) hk_flag(a.err, hk::kErrLaneRows, (unsigned)b);
       const Lane x = lane_at(s, b);
-      if (x.rows) n = steps_before(s.group, x.rows, x.pos0, tiles_of(s, x), tiles_of(s, x));
+      if (x.rows) n = units_before(s.group, x.rows, x.pos0, tiles_of(s, x), tiles_of(s, x));
     }
     return n * a.kv_heads;
   };
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
   int64_t total = 0;
   for (int b0 = 0; b0 < a.num_lanes; b0 += kThreads) {
     int64_t all;
-    scan_block(lane_steps(b0 + tid), &all);
+    scan_block(lane_units(b0 + tid), &all);
     total += all;
   }
   const int64_t ranges = min((int64_t)gridDim.x, total), cta = blockIdx.x;
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
   if (u0 < u1) {
     int64_t carry = 0;
     for (int b0 = 0; b0 < a.num_lanes; b0 += kThreads) {
-      const int64_t n = lane_steps(b0 + tid);
+      const int64_t n = lane_units(b0 + tid);
       int64_t all;
       const int64_t before = carry + scan_block(n, &all);
       if (before <= u0 && u0 < before + n) found[0] = before, found[1] = b0 + tid;
@@ -364,8 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
     // The tile in which the range begins: every thread tries its own.
     const int64_t into = u0 - found[0];
     for (int i = tid; i < w.tiles; i += kThreads) {
-      const int64_t from = steps_before(s.group, w.x.rows, w.x.pos0, i, w.tiles) * a.kv_heads;
-      if (from <= into && into < from + (int64_t)steps_of(s, w.x, i) * a.kv_heads) found[2] = i, found[3] = from - into;
+      const int64_t from = units_before(s.group, w.x.rows, w.x.pos0, i, w.tiles) * a.kv_heads;
+      if (from <= into && into < from + (int64_t)(steps_of(s, w.x, i) + kStart) * a.kv_heads) found[2] = i, found[3] = from - into;
     }
     __syncthreads();
     w.tile = (int)found[2];
@@ -381,50 +385,60 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lanes + half * 128, o_col = tmem + lanes + 256 + half * 128;
     uint8_t* q_rows = smem + L::kQ + half * L::kTile + (warp & 3) * 32 * 128;  // of this warp
-    uint32_t n_s = 0, n_o = 0, n_turn = 0, step = 0;
-    bool live = true;
-    while (live && w.next(s)) {
-      if (w.rows_left <= half * 128) {  // no rows for this half
-        step += w.last - w.first;
-        continue;
+    uint32_t n_s = 0, n_o = 0, n_turn = 0, step = 0, skipped = 0;
+    constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;  // lanes of a row of Q, rows a warp copies at once
+    const int part = lane % kLanes;
+    // The next problem of this half, and the copy of this warp's 32 rows of its Q, as they are, to their places.
+    int next_pos = 0;
+    auto next = [&]() {
+      while (true) {
+        if (!w.next(s)) return false;
+        if (w.rows_left > half * 128) break;
+        skipped += w.last - w.first;  // no rows for this half
       }
       const int r = half * 128 + row;
-      const bool both = w.rows_left > 128;
-      const bool on = r < w.rows_left;
-      const int pos = on ? a.positions[w.x.t0 + (w.row0 + r) / s.group] : INT32_MAX;
+      RowAt at(w.row0 + r - lane + lane / kLanes, s.group);
+      const RowAt by(kAtOnce, s.group);
+#pragma unroll 4
+      for (int i = 0; i < 32 / kAtOnce; ++i) {
+        const int wr = i * kAtOnce + lane / kLanes;
+        const bool on = r - lane + wr < w.rows_left;
+        const uint16_t* src = a.q + (on ? (w.x.t0 + at.t) * a.q_stride + (int64_t)(w.g * s.group + at.h) * D + part * 8 : 0);
+        const uint32_t dst = smem_u32(q_rows) + (part >> 3) * L::kHalf + wr * 128 + (((part & 7) ^ (wr & 7)) << 4);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+        at.add(by, s.group);
+      }
+      next_pos = r < w.rows_left ? a.positions[w.x.t0 + (w.row0 + r) / s.group] : INT32_MAX;
+      return true;
+    };
+    bool live = true, have = next();
+    step = skipped, skipped = 0;
+    while (live && have) {
+      // The current problem, as the walk moves on before its end.
+      const int first = w.first, last = w.last, r = half * 128 + row;
+      const bool both = w.rows_left > 128, on = r < w.rows_left;
+      const bool starts = w.first == 0, whole = starts && w.last == w.steps;
+      const int pos = next_pos;
+      const int pos_min = w.x.pos0 + (w.row0 + half * 128) / s.group;  // rows of a lane rise
+      const RowAt mine(w.row0 + r, s.group);
+      const int64_t y = (int64_t)(w.x.t0 + mine.t) * a.q_heads + w.g * s.group + mine.h;
+      // Q to fp16: each row scaled by a power of two, so that fp16 holds it exactly.  (A lane converts what it copied.)
       float rowf = 1.f;
-      // This warp's 32 rows of Q, D / 8 lanes to a row; each row scaled by a power of two so that fp16 holds it exactly.
-      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kBatch = 8;
-      const int part = lane % kLanes;
-      RowAt q_at(w.row0 + r - lane + lane / kLanes, s.group);
-      const RowAt q_step(kAtOnce, s.group);
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
-        uint4 u[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          u[i] = make_uint4(0, 0, 0, 0);
-          if (r - lane + (i0 + i) * kAtOnce + lane / kLanes < w.rows_left)
-            u[i] = *reinterpret_cast<const uint4*>(a.q + (w.x.t0 + q_at.t) * a.q_stride + (int64_t)(w.g * s.group + q_at.h) * D + part * 8);
-          q_at.add(q_step, s.group);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int wr = (i0 + i) * kAtOnce + lane / kLanes;  // row of the warp
-          float mine;
-          const uint4 x = scaled_row<kLanes>(u[i], s.is_f16, &mine);
-          *reinterpret_cast<uint4*>(q_rows + (part >> 3) * L::kHalf + wr * 128 + (((part & 7) ^ (wr & 7)) << 4)) = x;
-          const float back = __shfl_sync(0xffffffffu, mine, lane % kAtOnce * kLanes);
-          if (lane / kAtOnce == i0 + i) rowf = back;
-        }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+      for (int i = 0; i < 32 / kAtOnce; ++i) {
+        const int wr = i * kAtOnce + lane / kLanes;
+        uint4* at = reinterpret_cast<uint4*>(q_rows + (part >> 3) * L::kHalf + wr * 128 + (((part & 7) ^ (wr & 7)) << 4));
+        float back;
+        *at = scaled_row<kLanes>(*at, s.is_f16, &back);
+        back = __shfl_sync(0xffffffffu, back, lane % kAtOnce * kLanes);
+        if (lane / kAtOnce == i) rowf = back;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       warp_arrive(bar(kQFull, half));
-      // The smallest position of this half: rows of a lane rise.
-      const int pos_min = w.x.pos0 + (w.row0 + half * 128) / s.group;
 
       float m = kNoMax, l = 0.f;
-      for (int i = w.first; i < w.last; ++i, ++n_s, ++step) {
+      for (int i = first; i < last; ++i, ++n_s, ++step) {
         live = live && wait_bar(bar(kSFull, half), n_s & 1, abort, a.err, 0x70);
         live = __all_sync(0xffffffffu, live);
         if (!live) break;
@@ -436,6 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
           ++n_turn;
         }
         tc_fence_after();
+        if (i + 1 == last) have = next();  // this half's products with Q are complete: its next rows can come
         float v[128];
         tmem_ld128(s_col, v);
         constexpr int kGroups = kTok / kBox;
@@ -475,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
           const float m_new = over ? top : m, down = exp2_approx(m - m_new);
           m = m_new;
           l *= down;
-          if (i > w.first) {
+          if (i > first) {
 #pragma unroll 1
             for (int k = 0; k < D / 16; ++k) {
               float o[16];
@@ -521,46 +536,38 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
       if (!live) break;
       ++n_o;
       tc_fence_after();
-      // O leaves by way of this warp's rows of Q (both products are done with them), so that a row is written by
-      // neighbouring lanes: 32 dims at a time, as fp32 in a 128-byte line for each row, 16-byte parts swizzled.
-      const bool starts = w.first == 0, whole = starts && w.last == w.steps;
-      float* piece = s.part + ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (kRows * (D + 2));
-      const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      const RowAt out_step(4, s.group);
-      const RowAt out_first(w.row0 + r - lane + lane / 8, s.group);
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-      for (int k = 0; k < D / 32; ++k) {  // 32 dims: 128 bytes a row
-        float o[32];
-        tmem_ld32(o_col + 32 * k, o);
+        for (int k = 0; k < D / 32; ++k) {
+          float o[32];
+          tmem_ld32(o_col + 32 * k, o);
+          if (on) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          *reinterpret_cast<float4*>(q_rows + lane * 128 + ((e ^ (lane & 7)) << 4)) =
-              make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
-        __syncwarp();
-        RowAt at = out_first;
+            for (int e = 0; e < 32; ++e) o[e] *= inv;
+            uint4* to = reinterpret_cast<uint4*>(a.out + y * D + 32 * k);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // 4 rows at once, 8 lanes each
-          const int wr = i * 4 + lane / 8, qr = r - lane + wr;
-          const float4 x = *reinterpret_cast<const float4*>(q_rows + wr * 128 + (((lane & 7) ^ (wr & 7)) << 4));
-          if (qr < w.rows_left) {
-            if (whole) {
-              const int64_t y = (int64_t)(w.x.t0 + at.t) * a.q_heads + w.g * s.group + at.h;
-              *reinterpret_cast<uint2*>(a.out + y * D + 32 * k + (lane & 7) * 4) =
-                  s.is_f16 ? make_uint2(pack2<true>(x.x, x.y), pack2<true>(x.z, x.w)) : make_uint2(pack2<false>(x.x, x.y), pack2<false>(x.z, x.w));
-            } else {
-              *reinterpret_cast<float4*>(piece + qr * D + 32 * k + (lane & 7) * 4) = x;
-            }
+            for (int e = 0; e < 4; ++e) to[e] = s.is_f16 ? pack8<true>(o + 8 * e) : pack8<false>(o + 8 * e);
           }
-          at.add(out_step, s.group);
+          __syncwarp();
         }
-        __syncwarp();
+        if (on) a.lse[y] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
+      } else {
+        float* piece = s.part + ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (kRows * (D + 2));
+#pragma unroll 1
+        for (int k = 0; k < D / 32; ++k) {
+          float o[32];
+          tmem_ld32(o_col + 32 * k, o);
+          if (on) {
+            float4* to = reinterpret_cast<float4*>(piece + r * D + 32 * k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+          __syncwarp();
+        }
+        if (on) piece[kRows * D + r] = m, piece[kRows * (D + 1) + r] = l;
       }
-      if (on && whole) {
-        const int at = w.row0 + r, t = at / s.group;
-        a.lse[(int64_t)(w.x.t0 + t) * a.q_heads + w.g * s.group + at - t * s.group] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
-      } else if (on) {
-        piece[kRows * D + r] = m, piece[kRows * (D + 1) + r] = l;
-      }
+      step += skipped, skipped = 0;
       tc_fence_before();
     }
   } else {
