@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   const GqaArgs& a = s.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int G = a.kv_heads, group = s.group;
+  hk::let_next_grid_start();
   if (tid == 0) {
     for (int i = 0; i < kWarps; ++i) stop_s[i] = 0;
     for (int i = 0; i < kWarps * S; ++i) sm100::mbar_init(sm100::smem_u32(&full_s[0][0] + i), 1);
@@ -712,6 +713,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) gqa_merge_kernel(SplitArgs s
   const int first = blockIdx.x * kMergeWarps + warp;
   int pieces = 0;
   int64_t y = 0;  // (row, head) of the output
+  hk::wait_for_grid_before();
   const Rec rec = first < ctas ? s.rec[first] : Rec{-1, 0, 0, 0};
   if (rec.item >= 0) {
     const Item x = item_of<R, kSparse>(s, rec.item, false);
@@ -808,7 +810,7 @@ int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
   gqa_split_kernel<D, NT, kSparse><<<grid, kThreads, smem, stream>>>(s, kmap, vmap);
   HK_TRY_LAUNCH("gqa_split_kernel");
   if (grid > 1) {
-    gqa_merge_kernel<D, NT, kSparse><<<dim3((grid + kMergeWarps - 1) / kMergeWarps, 8 * NT), kMergeWarps * 32, 0, stream>>>(s, grid);
+    HK_TRY_CUDA(hk::launch_early(gqa_merge_kernel<D, NT, kSparse>, dim3((grid + kMergeWarps - 1) / kMergeWarps, 8 * NT), kMergeWarps * 32, 0, stream, s, grid));
     HK_TRY_LAUNCH("gqa_merge_kernel");
   }
   return HK_OK;

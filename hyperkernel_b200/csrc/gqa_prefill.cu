@@ -148,8 +148,8 @@ __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32
       : "r"(w));
 }
 
-// A wait of at most kTries tries (each of which may sleep for a while): short, as the kernel's code has to stay in the
-// instruction cache.  When it runs out it raises `abort`, which ends the others' waits.
+// A wait of at most kTries tries: short, as the kernel's code has to stay in the instruction cache (at 150 KB of code a step
+// took 1.2 times as long as at 100 KB).  When it runs out it raises `abort`, which ends the others' waits.
 constexpr uint32_t kTries = 1u << 22;
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort, unsigned long long* err, unsigned site) {
   uint32_t n = 0;
@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
   uint8_t* ctl = smem + L::kCtl;
   volatile int* abort = reinterpret_cast<volatile int*>(ctl + kAbort);
   const uint32_t base = smem_u32(smem), bars = smem_u32(ctl);
+  hk::let_next_grid_start();
   auto bar = [&](int off, int i = 0) { return bars + off + 8 * i; };
 
   if (base & 1023) {  // the swizzles count from 1 KB boundaries
@@ -512,8 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
           for (int e = 0; e < 32; e += 2) {
             const int t = 32 * j + e, k = t / kBox;
             const float f = factor(k), c = addend(k) - m;
+            const uint64_t x = fma2(pair(v[t], v[t + 1]), pair(f, f), pair(c, c));
             float x0, x1;
-            unpair(fma2(pair(v[t], v[t + 1]), pair(f, f), pair(c, c)), x0, x1);
+            unpair(x, x0, x1);
             x0 = exp2_approx(x0), x1 = exp2_approx(x1);
             sum = add2(sum, pair(x0, x1));
             p[e / 2] = pack2<true>(x0, x1);
@@ -754,6 +756,7 @@ __global__ void __launch_bounds__(256) gqa_prefill_merge_kernel(PrefillArgs s, i
   constexpr int P = D / 32;
   constexpr int64_t kPart = kRows * (D + 2);
   const GqaArgs& a = s.a;
+  hk::wait_for_grid_before();
   const Rec rec = s.rec[blockIdx.x];
   if (rec.lane < 0) return;
   const Lane x = lane_at(s, rec.lane);
@@ -795,7 +798,7 @@ int launch(PrefillArgs& s, int64_t steps, cudaStream_t stream) {
   gqa_prefill_kernel<D, kBox><<<grid, kThreads, L::kBytes, stream>>>(s, kmap, vmap);
   HK_TRY_LAUNCH("gqa_prefill_kernel");
   if (grid > 1) {
-    gqa_prefill_merge_kernel<D><<<dim3(grid, kRows / 8), 256, 0, stream>>>(s, grid);
+    HK_TRY_CUDA(hk::launch_early(gqa_prefill_merge_kernel<D>, dim3(grid, kRows / 8), 256, 0, stream, s, grid));
     HK_TRY_LAUNCH("gqa_prefill_merge_kernel");
   }
   return HK_OK;

@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(kScoreThreads) gqa_score_kernel(SelectArgs a) 
   __shared__ float warp_max[kScoreThreads / 32];
   __shared__ __align__(16) int8_t c8[256];
   const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  hk::let_next_grid_start();
   if (t >= a.cu[a.num_lanes]) return;
   const int n = blocks_of(a, t), from = blockIdx.z * kScoreBlocks, to = min(n - a.local, from + kScoreBlocks);
   if (n <= a.top || from >= to) return;
@@ -124,6 +125,7 @@ __global__ void __launch_bounds__(kThreads) gqa_select_kernel(SelectArgs a) {
   __shared__ int count_s[32];
   __shared__ int64_t sums_s[kWarps];
   const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  hk::wait_for_grid_before();
   if (t >= a.cu[a.num_lanes]) return;
   int32_t* list = a.blocks + ((int64_t)t * a.kv_heads + g) * a.top;
   const int n = blocks_of(a, t);
@@ -260,9 +262,15 @@ int hk_gqa_select_blocks(const uint16_t* q, int64_t q_stride, const int8_t* cent
     HK_TRY_LAUNCH("gqa_score_kernel");
   }
   const dim3 grid(num_tokens, kv_heads);
-  if (a.max_blocks <= 256 * kHold) gqa_select_kernel<256, true><<<grid, 256, 0, st>>>(a);
-  else if (a.max_blocks <= 1024 * kHold) gqa_select_kernel<1024, true><<<grid, 1024, 0, st>>>(a);
-  else gqa_select_kernel<1024, false><<<grid, 1024, 0, st>>>(a);
+  const bool early = a.max_blocks > top_blocks;  // behind the scores
+  auto select = [&](auto kernel, int threads) -> cudaError_t {
+    if (early) return hk::launch_early(kernel, grid, threads, 0, st, a);
+    kernel<<<grid, threads, 0, st>>>(a);
+    return cudaSuccess;
+  };
+  if (a.max_blocks <= 256 * kHold) HK_TRY_CUDA(select(gqa_select_kernel<256, true>, 256));
+  else if (a.max_blocks <= 1024 * kHold) HK_TRY_CUDA(select(gqa_select_kernel<1024, true>, 1024));
+  else HK_TRY_CUDA(select(gqa_select_kernel<1024, false>, 1024));
   HK_TRY_LAUNCH("gqa_select_kernel");
   return HK_OK;
 }
