@@ -7,6 +7,7 @@ sm_100 part, calls raise HKError.  torch is used only for device memory and stre
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import re
 from pathlib import Path
@@ -150,8 +151,9 @@ def ptr(t):
 
 
 def stream_ptr(stream=None):
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())  # the current stream, without its Python object
 
 
 def call(name: str, *args) -> None:
@@ -330,33 +332,34 @@ def mla_partial(q, kv_cache, block_table, cu_seqlens, positions, kv_begin, kv_en
 # ---- GQA over the block-scaled 8-bit cache -----------------------------------------------
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # HK_BF16, HK_F16
+_I32, _F32, _U8, _I8 = torch.int32, torch.float32, torch.uint8, torch.int8
 
 
-def _rows(t, like=None):
+def _rows(t):
     """(address, row stride in elements) of a [rows, heads, dim] tensor whose rows may be slices of
-    wider ones; with `like`, also of its shape, type and device."""
+    wider ones."""
     T, h, d = t.shape
-    s = t.stride()
-    if like is not None and (t.shape, t.dtype, t.device) != (like.shape, like.dtype, like.device):
-        raise ValueError(f"expected a {like.dtype} tensor of shape {tuple(like.shape)} on {like.device}")
-    if T > 1 and h > 0:
-        if s[2] != 1 or (s[1] != d and h > 1):
-            raise ValueError("heads of a row must lie side by side")
-        return t.data_ptr(), s[0]
-    if h > 0 and (s[2] != 1 or (s[1] != d and h > 1)):
-        raise ValueError("heads of a row must lie side by side")
-    return t.data_ptr(), h * d
+    s0, s1, s2 = t.stride()
+    if h > 0 and (s2 != 1 or (s1 != d and h > 1)):
+        raise ValueError("the heads of a row must lie side by side")
+    return t.data_ptr(), s0 if T > 1 and h > 0 else h * d
 
 
-def _here(dtype, *tensors):
-    """The HK_BF16 / HK_F16 code, after checking that every tensor is on the current device."""
-    if dtype not in _DTYPES:
-        raise TypeError(f"expected bfloat16 or float16, got {dtype}")
+def _code(t):
+    """The HK_BF16 / HK_F16 code of a tensor."""
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise TypeError(f"expected bfloat16 or float16, got {t.dtype}") from None
+
+
+def _here(*tensors):
+    """The current device, after checking that every tensor is on it."""
     dev = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
-    return _DTYPES[dtype]
+    return dev
 
 
 def _typed(t, dtype, name):
@@ -365,6 +368,16 @@ def _typed(t, dtype, name):
     if t.dtype != dtype or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous {dtype} tensor")
     return t.data_ptr()
+
+
+def _output(out, like, shape):
+    """(tensor, address, row stride) of an output of `like`'s type: a new one unless given."""
+    if out is None:
+        out = like.new_empty(shape)
+        return out, out.data_ptr(), shape[1] * shape[2]
+    if out.shape != shape or out.dtype != like.dtype:
+        raise ValueError(f"expected a {like.dtype} output of shape {tuple(shape)}")
+    return (out, *_rows(out))
 
 
 def qk_norm_rope(q, k, positions, table, q_gain=None, k_gain=None, interleaved=False, eps=1e-6,
@@ -377,87 +390,92 @@ def qk_norm_rope(q, k, positions, table, q_gain=None, k_gain=None, interleaved=F
     G = k.shape[1]
     if k.shape != (T, G, D) or k.dtype != q.dtype or positions.shape[0] < T or table.dim() != 2:
         raise ValueError("q, k, positions and table do not fit together")
-    for w in (q_gain, k_gain):
-        if w is not None and w.shape != (D,):
-            raise ValueError(f"a gain has {D} elements")
-    dt = _here(q.dtype, q, k, positions, table, q_gain, k_gain, q_out, k_out)
-    if q_out is None:
-        q_out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
-    if k_out is None:
-        k_out = torch.empty((T, G, D), dtype=q.dtype, device=q.device)
-    (qp, qs), (kp, ks), (yp, ys), (zp, zs) = _rows(q), _rows(k), _rows(q_out, q), _rows(k_out, k)
-    call("hk_qk_norm_rope", qp, qs, kp, ks, _typed(q_gain, q.dtype, "q_gain"), _typed(k_gain, q.dtype, "k_gain"),
-         _typed(table, torch.float32, "table"), table.shape[0], table.shape[1], int(interleaved),
-         _typed(positions, torch.int32, "positions"), T, H, G, D, eps, dt, yp, ys, zp, zs, stream_ptr(stream))
+    if (q_gain is not None and q_gain.shape != (D,)) or (k_gain is not None and k_gain.shape != (D,)):
+        raise ValueError(f"a gain has {D} elements")
+    _here(q, k, positions, table, q_gain, k_gain, q_out, k_out)
+    dt = q.dtype
+    q_out, yp, ys = _output(q_out, q, (T, H, D))
+    k_out, zp, zs = _output(k_out, k, (T, G, D))
+    qp, qs = _rows(q)
+    kp, ks = _rows(k)
+    call("hk_qk_norm_rope", qp, qs, kp, ks, _typed(q_gain, dt, "q_gain"), _typed(k_gain, dt, "k_gain"),
+         _typed(table, _F32, "table"), table.shape[0], table.shape[1], int(interleaved),
+         _typed(positions, _I32, "positions"), T, H, G, D, eps, _code(q), yp, ys, zp, zs, stream_ptr(stream))
     return q_out, k_out
 
 
 def _gqa_cache(k_cache, v_cache, k_scale, v_scale):
-    """(pages, KV heads, page rows, dim) of a cache after checking its four arrays."""
-    N, G, R, D = k_cache.shape
-    if v_cache.shape != k_cache.shape or k_scale.shape != (N, G) or v_scale.shape != (N, G):
+    """(pages, KV heads, page rows, dim) and the addresses of a cache, after checking its four arrays."""
+    shape = N, G, R, D = k_cache.shape
+    if v_cache.shape != shape or k_scale.shape != (N, G) or v_scale.shape != (N, G):
         raise ValueError("k_cache, v_cache [pages, kv_heads, page, dim] and their scales [pages, kv_heads] do not fit together")
-    return N, G, R, D
+    return N, G, R, D, (_typed(k_cache, _U8, "k_cache"), _typed(v_cache, _U8, "v_cache"),
+                        _typed(k_scale, _F32, "k_scale"), _typed(v_scale, _F32, "v_scale"))
 
 
 def gqa_append_fp8(k_new, v_new, slot_mapping, k_cache, v_cache, k_scale, v_scale, centroids=None,
                    centroid_scale=None, stream=None):
     """Appends rows to the block-scaled e4m3 cache (uint8 [pages, kv_heads, page, dim], fp32 scales
     [pages, kv_heads]) and, when given, the int8 centroids of the pages that become full."""
-    N, G, R, D = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
+    N, G, R, D, cache = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
     T = k_new.shape[0]
     if k_new.shape != (T, G, D) or v_new.shape != (T, G, D) or v_new.dtype != k_new.dtype or slot_mapping.shape[0] < T:
         raise ValueError("k_new, v_new [rows, kv_heads, dim] and slot_mapping do not fit the cache")
-    if centroids is not None and (centroids.shape != (N, G, D) or centroid_scale is None or centroid_scale.shape != (N, G)):
+    if (centroids is None) != (centroid_scale is None) or (
+            centroids is not None and (centroids.shape != (N, G, D) or centroid_scale.shape != (N, G))):
         raise ValueError("centroids [pages, kv_heads, dim] need centroid_scale [pages, kv_heads]")
-    dt = _here(k_new.dtype, k_new, v_new, slot_mapping, k_cache, v_cache, k_scale, v_scale, centroids, centroid_scale)
-    (kp, ks), (vp, vs) = _rows(k_new), _rows(v_new)
-    call("hk_gqa_append_fp8", kp, ks, vp, vs, dt, _typed(slot_mapping, torch.int32, "slot_mapping"), T, G, D, R, N,
-         _typed(k_cache, torch.uint8, "k_cache"), _typed(v_cache, torch.uint8, "v_cache"),
-         _typed(k_scale, torch.float32, "k_scale"), _typed(v_scale, torch.float32, "v_scale"),
-         _typed(centroids, torch.int8, "centroids"), _typed(centroid_scale, torch.float32, "centroid_scale"), stream_ptr(stream))
+    _here(k_new, v_new, slot_mapping, k_cache, v_cache, k_scale, v_scale, centroids, centroid_scale)
+    kp, ks = _rows(k_new)
+    vp, vs = _rows(v_new)
+    call("hk_gqa_append_fp8", kp, ks, vp, vs, _code(k_new), _typed(slot_mapping, _I32, "slot_mapping"), T, G, D, R, N,
+         *cache, _typed(centroids, _I8, "centroids"), _typed(centroid_scale, _F32, "centroid_scale"), stream_ptr(stream))
 
 
 def gqa_fp8_workspace_size(num_tokens, q_heads, kv_heads, head_dim) -> int:
     return lib().hk_gqa_fp8_workspace_size(num_tokens, q_heads, kv_heads, head_dim)
 
 
-def _gqa_io(q, G, D, out, lse, workspace):
+@functools.lru_cache(maxsize=256)
+def _gqa_scratch(device, *sizes):
+    return gqa_fp8_workspace_size(*sizes)  # of the sizes and the device's SMs alone
+
+
+def _gqa_io(q, G, D, out, lse, workspace, dev):
     T, H, d = q.shape
     if d != D:
         raise ValueError(f"q has heads of {d} dims, the cache of {D}")
     if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((T, H, D))
+    elif out.shape != (T, H, D):
+        raise ValueError("out does not fit q")
     if lse is None:
-        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
-    if out.shape != q.shape or lse.shape != (T, H):
-        raise ValueError("out and lse do not fit q")
+        lse = q.new_empty((T, H), dtype=_F32)
+    elif lse.shape != (T, H):
+        raise ValueError("lse does not fit q")
     if workspace is None:
-        workspace = torch.empty(gqa_fp8_workspace_size(T, H, G, D), dtype=torch.uint8, device=q.device)
-    return out, lse, workspace
+        workspace = q.new_empty(_gqa_scratch(dev, T, H, G, D), dtype=_U8)
+    return out, lse, workspace, (_typed(out, q.dtype, "out"), _typed(lse, _F32, "lse"), _typed(workspace, _U8, "workspace"), workspace.shape[0])
 
 
 def _lanes(block_table, cu_seqlens, positions, T):
     if block_table.dim() != 2 or cu_seqlens.shape[0] != block_table.shape[0] + 1 or positions.shape[0] < T:
         raise ValueError("block_table [lanes, pages], cu_seqlens [lanes + 1] and positions do not fit together")
-    return (_typed(block_table, torch.int32, "block_table"), block_table.shape[1],
-            _typed(cu_seqlens, torch.int32, "cu_seqlens"), _typed(positions, torch.int32, "positions"))
+    return (_typed(block_table, _I32, "block_table"), block_table.shape[1], _typed(cu_seqlens, _I32, "cu_seqlens"),
+            _typed(positions, _I32, "positions"))
 
 
 def gqa_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, max_rows,
                    max_kv_len, scale, out=None, lse=None, workspace=None, stream=None):
     """Ragged paged attention over the block-scaled cache of `gqa_append_fp8`: every lane's rows
     (at most max_rows) attend the lane's KV rows up to their positions.  Returns (out, lse)."""
-    N, G, R, D = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
+    N, G, R, D, cache = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
     T, H, _ = q.shape
-    dt = _here(q.dtype, q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, out, lse, workspace)
-    out, lse, workspace = _gqa_io(q, G, D, out, lse, workspace)
-    qp, qs = _rows(q)
-    bt, stride, cu, pos = _lanes(block_table, cu_seqlens, positions, T)
-    call("hk_gqa_decode_fp8", qp, qs, _typed(k_cache, torch.uint8, "k_cache"), _typed(v_cache, torch.uint8, "v_cache"),
-         _typed(k_scale, torch.float32, "k_scale"), _typed(v_scale, torch.float32, "v_scale"), bt, stride, cu, pos,
-         block_table.shape[0], T, H, G, D, R, N, max_rows, max_kv_len, scale, dt, _typed(out, q.dtype, "out"),
-         _typed(lse, torch.float32, "lse"), ptr(workspace), workspace.numel(), stream_ptr(stream))
+    lanes = _lanes(block_table, cu_seqlens, positions, T)
+    dev = _here(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, out, lse, workspace)
+    dt = _code(q)
+    out, lse, workspace, io = _gqa_io(q, G, D, out, lse, workspace, dev)
+    call("hk_gqa_decode_fp8", *_rows(q), *cache, *lanes, block_table.shape[0], T, H, G, D, R, N, max_rows, max_kv_len,
+         scale, dt, *io, stream_ptr(stream))
     return out, lse
 
 
@@ -469,37 +487,34 @@ def gqa_select_blocks(q, centroids, centroid_scale, block_table, cu_seqlens, pos
     T, H, d = q.shape
     if d != D or centroid_scale.shape != (N, G):
         raise ValueError("q, centroids and centroid_scale do not fit together")
-    dt = _here(q.dtype, q, centroids, centroid_scale, block_table, cu_seqlens, positions, blocks, workspace)
+    lanes = _lanes(block_table, cu_seqlens, positions, T)
+    _here(q, centroids, centroid_scale, block_table, cu_seqlens, positions, blocks, workspace)
     if blocks is None:
-        blocks = torch.empty((T, G, top_blocks), dtype=torch.int32, device=q.device)
+        blocks = q.new_empty((T, G, top_blocks), dtype=_I32)
     elif blocks.shape != (T, G, top_blocks):
         raise ValueError("blocks must be [T, kv_heads, top_blocks]")
     if workspace is None:
-        workspace = torch.empty(lib().hk_gqa_select_workspace_size(T, G, page_size, max_kv_len), dtype=torch.uint8, device=q.device)
-    qp, qs = _rows(q)
-    bt, stride, cu, pos = _lanes(block_table, cu_seqlens, positions, T)
-    call("hk_gqa_select_blocks", qp, qs, _typed(centroids, torch.int8, "centroids"),
-         _typed(centroid_scale, torch.float32, "centroid_scale"), bt, stride, cu, pos, block_table.shape[0], T, H, G, D,
-         page_size, N, max_kv_len, top_blocks, sink, local, dt, _typed(blocks, torch.int32, "blocks"), ptr(workspace),
-         workspace.numel(), stream_ptr(stream))
+        workspace = q.new_empty(lib().hk_gqa_select_workspace_size(T, G, page_size, max_kv_len), dtype=_U8)
+    call("hk_gqa_select_blocks", *_rows(q), _typed(centroids, _I8, "centroids"),
+         _typed(centroid_scale, _F32, "centroid_scale"), *lanes, block_table.shape[0], T, H, G, D, page_size, N,
+         max_kv_len, top_blocks, sink, local, _code(q), _typed(blocks, _I32, "blocks"),
+         _typed(workspace, _U8, "workspace"), workspace.shape[0], stream_ptr(stream))
     return blocks
 
 
 def gqa_sparse_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, blocks, scale,
                    out=None, lse=None, workspace=None, stream=None):
     """`gqa_decode_fp8` over the listed blocks of each row and KV head.  Returns (out, lse)."""
-    N, G, R, D = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
+    N, G, R, D, cache = _gqa_cache(k_cache, v_cache, k_scale, v_scale)
     T, H, _ = q.shape
     if blocks.dim() != 3 or blocks.shape[:2] != (T, G):
         raise ValueError("blocks must be [T, kv_heads, top_blocks]")
-    dt = _here(q.dtype, q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, blocks, out, lse, workspace)
-    out, lse, workspace = _gqa_io(q, G, D, out, lse, workspace)
-    qp, qs = _rows(q)
-    bt, stride, cu, pos = _lanes(block_table, cu_seqlens, positions, T)
-    call("hk_gqa_sparse_fp8", qp, qs, _typed(k_cache, torch.uint8, "k_cache"), _typed(v_cache, torch.uint8, "v_cache"),
-         _typed(k_scale, torch.float32, "k_scale"), _typed(v_scale, torch.float32, "v_scale"), bt, stride, cu, pos,
-         _typed(blocks, torch.int32, "blocks"), blocks.shape[2], block_table.shape[0], T, H, G, D, R, N, scale, dt,
-         _typed(out, q.dtype, "out"), _typed(lse, torch.float32, "lse"), ptr(workspace), workspace.numel(), stream_ptr(stream))
+    lanes = _lanes(block_table, cu_seqlens, positions, T)
+    dev = _here(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, blocks, out, lse, workspace)
+    dt = _code(q)
+    out, lse, workspace, io = _gqa_io(q, G, D, out, lse, workspace, dev)
+    call("hk_gqa_sparse_fp8", *_rows(q), *cache, *lanes, _typed(blocks, _I32, "blocks"), blocks.shape[2],
+         block_table.shape[0], T, H, G, D, R, N, scale, dt, *io, stream_ptr(stream))
     return out, lse
 
 

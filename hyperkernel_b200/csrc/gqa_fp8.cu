@@ -354,7 +354,7 @@ __device__ __forceinline__ int64_t block_excl_scan(int64_t v, int64_t* sums, int
 
 template <int D, int NT>
 constexpr int split_smem() {
-  constexpr int ring = kWarps * stages(D, NT) * 32 * D, joined = kWarps / 2 * NT * (D / 16) * 32 * 16;  // O of half the warps
+  constexpr int ring = kWarps * stages(D, NT) * 32 * D, joined = kWarps * NT * (D / 16) * 32 * 16;  // O of every warp
   static_assert(stages(D, NT) >= 2 && stages(D, NT) <= kLook && joined <= ring, "ring");
   return ring + 1024;  // lines are swizzled from 1 KB boundaries
 }
@@ -366,10 +366,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   extern __shared__ uint8_t dyn_raw[];
   uint8_t* dyn = dyn_raw + (1024 - (__cvta_generic_to_shared(dyn_raw) & 1023)) % 1024;
   constexpr int S = stages(D, NT);
-  float4* o_s = reinterpret_cast<float4*>(dyn);  // [kWarps / 2][NT * D / 16][32], over the ring once it is read
+  float4* o_s = reinterpret_cast<float4*>(dyn);  // [kWarps][D / 16][NT][32], over the ring once it is read
   __shared__ __align__(16) uint4 q_s[NT * (D / 32) * 32];  // B fragments of Q: [N tile][two k steps][lane]
   __shared__ float rowf_s[R], m_s[kWarps][R], l_s[kWarps][R];
   __shared__ int pos_s[R];
+  __shared__ float inv_s[R];
+  __shared__ int64_t row_s[R];
   __shared__ int64_t scan_s[kWarps];
   __shared__ int64_t at_s;
   __shared__ int item_s;
@@ -393,16 +395,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   const Offsets<D> at(r, c);
   // (the barriers are seen by all after the scan's first __syncthreads)
 
-  // This CTA's range of units, and the item it begins in.
-  int64_t total = 0;
+  // This CTA's range of units, and the item it begins in.  (With more items than threads the scan is run again to find it.)
+  int64_t total = 0, mine = 0, before = 0;
   for (int base = 0; base < s.items; base += kThreads) {
     const int i = base + tid;
-    int64_t n = 0, all;
+    int64_t all;
+    mine = 0;
     if (i < s.items) {
       const Item x = item_of<R, kSparse>(s, i, blockIdx.x == 0);
-      n = x.nu * x.tiles * G;
+      mine = x.nu * x.tiles * G;
     }
-    block_excl_scan(n, scan_s, &all);
+    before = total + block_excl_scan(mine, scan_s, &all);
     total += all;
   }
   // One range for each resident CTA: two to four ranges, which even out the SMs, measured 4 to 11% slower
@@ -411,18 +414,23 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   const int64_t u0 = cta < ranges ? total * cta / ranges : 0, u1 = cta < ranges ? total * (cta + 1) / ranges : 0;
   Rec rec = {-1, 0, 0, 0};
   if (u0 < u1) {
-    int64_t carry = 0;
-    for (int base = 0; base < s.items; base += kThreads) {
-      const int i = base + tid;
-      int64_t n = 0, all;
-      if (i < s.items) {
-        const Item x = item_of<R, kSparse>(s, i, false);
-        n = x.nu * x.tiles * G;
+    if (s.items <= kThreads) {
+      if (before <= u0 && u0 < before + mine) item_s = tid, at_s = before;
+    } else {
+      int64_t carry = 0;
+      for (int base = 0; base < s.items; base += kThreads) {
+        const int i = base + tid;
+        int64_t all;
+        mine = 0;
+        if (i < s.items) {
+          const Item x = item_of<R, kSparse>(s, i, false);
+          mine = x.nu * x.tiles * G;
+        }
+        before = carry + block_excl_scan(mine, scan_s, &all);
+        if (before <= u0 && u0 < before + mine) item_s = i, at_s = before;
+        carry += all;
+        if (carry > u0) break;
       }
-      const int64_t before = carry + block_excl_scan(n, scan_s, &all);
-      if (before <= u0 && u0 < before + n) item_s = i, at_s = before;
-      carry += all;
-      if (carry > u0) break;
     }
     __syncthreads();
     int i = item_s;
@@ -440,57 +448,34 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
       const int tok0 = first * kUnit, tok1 = min(x.len, last * kUnit);
       const int lane_b = kSparse ? hk::lane_of_row(a.cu, a.num_lanes, x.t0) : i;
       __syncthreads();
-      // Query rows: scaled by a power of two so that fp16 holds them exactly, in the order of the fragments.
-      for (int n = warp; n < R; n += kWarps) {
-        const int row = row0 + n;
-        const bool on = row < x.rows * group;
-        const int t = x.t0 + (on ? row / group : 0), h = g * group + row % group;
-        float f[D / 32];
-        float top = 0.f;
+      // The query rows of this warp, asked for now and used after the lookups below: lane y finds row warp + kWarps y.
+      constexpr int kMine = R / kWarps;
+      uint32_t qw[kMine][D / 64];
+      int my_pos = INT32_MAX;
+      {
+        if (tid < R && row0 + tid < x.rows * group) my_pos = a.positions[x.t0 + (row0 + tid) / group];
+        const int row = row0 + warp + kWarps * (lane % kMine);
+        const int t = row / group;
+        const int64_t at = row < x.rows * group ? (x.t0 + t) * a.q_stride + (int64_t)(g * group + row - t * group) * D : -1;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          f[e] = 0.f;
-          if (on) {
-            const uint16_t w = a.q[t * a.q_stride + (int64_t)h * D + lane * (D / 32) + e];
-            f[e] = s.is_f16 ? __half2float(*reinterpret_cast<const __half*>(&w)) : bf16_bits_to_f32(w);
+        for (int y = 0; y < kMine; ++y) {
+          const int64_t from = __shfl_sync(0xffffffffu, at, y);
+#pragma unroll
+          for (int e = 0; e < D / 64; ++e) qw[y][e] = 0;
+          if (from >= 0) {
+            const uint16_t* src = a.q + from + lane * (D / 32);
+            if (D == 64) {
+              qw[y][0] = *reinterpret_cast<const uint32_t*>(src);
+            } else if (D == 128) {
+              const uint2 u = *reinterpret_cast<const uint2*>(src);
+              qw[y][0] = u.x, qw[y][1 % (D / 64)] = u.y;
+            } else {
+              const uint4 u = *reinterpret_cast<const uint4*>(src);
+              qw[y][0] = u.x, qw[y][1 % (D / 64)] = u.y, qw[y][2 % (D / 64)] = u.z, qw[y][3 % (D / 64)] = u.w;
+            }
           }
-          top = fmaxf(top, fabsf(f[e]));
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const int ex = (int)((__float_as_uint(top) >> 23) & 255);  // 0: zero or subnormal, 255: not finite
-        const int up = ex == 255 ? 0 : min(134 - ex, 120);
-        const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          const int d = lane * (D / 32) + e;
-          const int part = d / 16, half = D == 256 ? part & 7 : part;  // the inverse of k_part
-          const int cc = D == 64 ? part : D == 128 ? part >> 1 : (half & 1) | (half >> 2) << 1;
-          const int i = D == 64 ? 0 : D == 128 ? part & 1 : (part >> 3) * 2 + (half >> 1 & 1);
-          const int k = i * 4 + (d % 16) / 4;
-          reinterpret_cast<__half*>(q_s + ((n >> 3) * (D / 32) + k / 2) * 32 + (n & 7) * 4 + cc)[(k & 1) * 4 + (d & 3)] = __float2half_rn(f[e] * mul);
-        }
-        if (lane == 0) {
-          rowf_s[n] = __uint_as_float((uint32_t)(127 - up) << 23);
-          pos_s[n] = on ? a.positions[t] : INT32_MAX;
         }
       }
-      __syncthreads();
-      float rowf[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) rowf[n][0] = rowf_s[n * 8 + 2 * c], rowf[n][1] = rowf_s[n * 8 + 2 * c + 1];
-      const int pos_min = kSparse ? x.pos : pos_s[0];  // the first row's: positions rise
-      const int len = kSparse ? x.pos + 1 : x.len;
-
-      State<D, NT> st;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        st.m[n][0] = st.m[n][1] = kNoMax;
-        st.l[n][0] = st.l[n][1] = 0.f;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) st.o[j][n][0] = st.o[j][n][1] = st.o[j][n][2] = st.o[j][n][3] = 0.f;
-      }
-
       // This warp's chunks: tokens tok0 + 16 warp + kUnit e.
       const int32_t* row_bt = a.bt + (int64_t)lane_b * a.bt_stride;
       const int32_t* list = kSparse ? a.blocks + ((int64_t)x.t0 * G + g) * a.top : nullptr;
@@ -520,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
               line = (int32_t)((at * a.page_size + r16) * D / 128);
               y.kf = a.ks[at] * (a.scale * kLog2e);
               const float vs = fmaxf(a.vs[at], 7.8886090522101181e-31f);
-              y.lsv = log2f(vs), y.isv = 1.f / vs;
+              y.lsv = __log2f(vs), y.isv = __frcp_rn(vs);
             }
           }
           line_s[warp][(e0 + lane) % (2 * kLook)] = line;
@@ -542,10 +527,53 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
         fill = fill + 1 == S ? 0 : fill + 1;
         ++filled;
       };
-      look(0);
-      look(kLook);
+#pragma unroll 1
+      for (int e = 0; e < 2 * kLook; e += kLook) look(e);
 #pragma unroll 1
       for (int e = 0; e < S - 1; ++e) ask(e);
+      // Query rows: scaled by a power of two so that fp16 holds them exactly, in the order of the fragments.
+#pragma unroll
+      for (int y = 0; y < kMine; ++y) {
+        const int n = warp + kWarps * y;
+        float f[D / 32], top = 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const uint16_t bits = (uint16_t)(qw[y][e / 2] >> (16 * (e & 1)));
+          f[e] = s.is_f16 ? __half2float(__ushort_as_half(bits)) : bf16_bits_to_f32(bits);
+          top = fmaxf(top, fabsf(f[e]));
+        }
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // (magnitudes: their bits are in order)
+        const int ex = (int)((__float_as_uint(top) >> 23) & 255);  // 0: zero or subnormal, 255: not finite
+        const int up = ex == 255 ? 0 : min(134 - ex, 120);
+        const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const int d = lane * (D / 32) + e;
+          const int part = d / 16, half = D == 256 ? part & 7 : part;  // the inverse of k_part
+          const int cc = D == 64 ? part : D == 128 ? part >> 1 : (half & 1) | (half >> 2) << 1;
+          const int i = D == 64 ? 0 : D == 128 ? part & 1 : (part >> 3) * 2 + (half >> 1 & 1);
+          const int k = i * 4 + (d % 16) / 4;
+          reinterpret_cast<__half*>(q_s + ((n >> 3) * (D / 32) + k / 2) * 32 + (n & 7) * 4 + cc)[(k & 1) * 4 + (d & 3)] = __float2half_rn(f[e] * mul);
+        }
+        if (lane == 0) rowf_s[n] = __uint_as_float((uint32_t)(127 - up) << 23);
+      }
+      if (tid < R) pos_s[tid] = my_pos;
+      __syncthreads();
+      float rowf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) rowf[n][0] = rowf_s[n * 8 + 2 * c], rowf[n][1] = rowf_s[n * 8 + 2 * c + 1];
+      const int pos_min = kSparse ? x.pos : pos_s[0];  // the first row's: positions rise
+      const int len = kSparse ? x.pos + 1 : x.len;
+
+      State<D, NT> st;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        st.m[n][0] = st.m[n][1] = kNoMax;
+        st.l[n][0] = st.l[n][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) st.o[j][n][0] = st.o[j][n][1] = st.o[j][n][2] = st.o[j][n][3] = 0.f;
+      }
+
 #pragma unroll 1
       for (int e = 0; e < nchunk; ++e) {
         if (e > 0 && e % kLook == 0) look(e + kLook);
@@ -582,7 +610,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
         __syncwarp();
       }
 
-      // Join the warps: maxima through shared memory, then O pairwise (4 + 4, 2 + 2, 1 + 1).
+      // Join the warps through shared memory (over the ring, which is read): each warp's maxima and sums, then its O under the
+      // common maximum; the threads add the warps' parts in order and write the rows.  (The code after the loop is kept
+      // short: a small call's time is in good part that of fetching it.)
+      const bool starts = first == 0, ends = last == x.nu;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -593,73 +624,61 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
           if (r == 0) m_s[warp][n * 8 + 2 * c + e] = st.m[n][e], l_s[warp][n * 8 + 2 * c + e] = l;
         }
       __syncthreads();
-      float top[NT][2], sum[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = n * 8 + 2 * c + e;
-          float m = kNoMax, l = 0.f;
+          float m = kNoMax;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) m = fmaxf(m, m_s[w][row]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) l += l_s[w][row] * exp2_approx(m_s[w][row] - m);
-          top[n][e] = m, sum[n][e] = l;
-          const float f = exp2_approx(st.m[n][e] - m);
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) st.o[j][n][e] *= f, st.o[j][n][e + 2] *= f;
+          f[e] = exp2_approx(st.m[n][e] - m);
         }
 #pragma unroll
-      for (int half = kWarps / 2; half > 0; half >>= 1) {
-        if (warp >= half && warp < 2 * half) {
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              o_s[(((warp - half) * (D / 16) + j) * NT + n) * 32 + lane] = make_float4(st.o[j][n][0], st.o[j][n][1], st.o[j][n][2], st.o[j][n][3]);
-        }
-        __syncthreads();
-        if (warp < half) {
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float4 y = o_s[((warp * (D / 16) + j) * NT + n) * 32 + lane];
-              st.o[j][n][0] += y.x, st.o[j][n][1] += y.y, st.o[j][n][2] += y.z, st.o[j][n][3] += y.w;
-            }
-        }
-        __syncthreads();
+        for (int j = 0; j < D / 16; ++j)
+          o_s[((warp * (D / 16) + j) * NT + n) * 32 + lane] =
+              make_float4(st.o[j][n][0] * f[0], st.o[j][n][1] * f[1], st.o[j][n][2] * f[0], st.o[j][n][3] * f[1]);
       }
-      const bool starts = first == 0, ends = last == x.nu;
-      if (warp == 0) {
-        float* part = s.part + ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (R * D + 2 * R);
+      float* part = s.part + ((int64_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (R * D + 2 * R);
+      const bool whole = starts && ends;
+      if (tid < R) {  // a row's denominator, and where it goes
+        float m = kNoMax, l = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, m_s[w][tid]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = n * 8 + 2 * c + e, at = row0 + row;
-            if (starts && ends) {
-              if (at >= x.rows * group) continue;
-              const int64_t y = (int64_t)(x.t0 + at / group) * a.q_heads + g * group + at % group;
-              const float inv = sum[n][e] == 0.f ? 0.f : 1.f / sum[n][e];
+        for (int w = 0; w < kWarps; ++w) l += l_s[w][tid] * exp2_approx(m_s[w][tid] - m);
+        const int at = row0 + tid;
+        int64_t y = -1;
+        if (at < x.rows * group) {
+          y = (int64_t)(x.t0 + at / group) * a.q_heads + g * group + at % group;
+          if (whole) a.lse[y] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
+          else part[R * D + tid] = m, part[R * D + R + tid] = l;
+        }
+        row_s[tid] = y;
+        inv_s[tid] = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int k = tid; k < D / 32 * NT * 32; k += kThreads) {  // four dims of two rows
+        const int ln = k & 31, n = k / 32 % NT, w = k / 32 / NT, cc = ln & 3, d = v_dim<D>(ln >> 2, w);
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
 #pragma unroll
-              for (int w = 0; w < D / 32; ++w) {
-                const float o0 = st.o[2 * w][n][e] * inv, o1 = st.o[2 * w][n][e + 2] * inv, o2 = st.o[2 * w + 1][n][e] * inv,
-                            o3 = st.o[2 * w + 1][n][e + 2] * inv;
-                uint2 u;
-                if (s.is_f16) u = make_uint2(pack2<true>(o0, o1), pack2<true>(o2, o3));
-                else u = make_uint2(pack2<false>(o0, o1), pack2<false>(o2, o3));
-                *reinterpret_cast<uint2*>(a.out + y * D + v_dim<D>(r, w)) = u;
-              }
-              if (r == 0) a.lse[y] = sum[n][e] == 0.f ? -INFINITY : fmaf(top[n][e], kLn2, logf(sum[n][e]));
-            } else {
-#pragma unroll
-              for (int w = 0; w < D / 32; ++w)
-                *reinterpret_cast<float4*>(part + row * D + v_dim<D>(r, w)) =
-                    make_float4(st.o[2 * w][n][e], st.o[2 * w][n][e + 2], st.o[2 * w + 1][n][e], st.o[2 * w + 1][n][e + 2]);
-              if (r == 0) part[R * D + row] = top[n][e], part[R * D + R + row] = sum[n][e];
-            }
-          }
+        for (int e = 0; e < kWarps; ++e) {
+          const float4 p = o_s[((e * (D / 16) + 2 * w) * NT + n) * 32 + ln], q = o_s[((e * (D / 16) + 2 * w + 1) * NT + n) * 32 + ln];
+          u.x += p.x, u.y += p.z, u.z += q.x, u.w += q.z;
+          v.x += p.y, v.y += p.w, v.z += q.y, v.w += q.w;
+        }
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e, u = v) {
+          const int row = n * 8 + 2 * cc + e;
+          const int64_t y = row_s[row];
+          if (y < 0) continue;
+          const float f = inv_s[row];
+          if (!whole) *reinterpret_cast<float4*>(part + row * D + d) = u;
+          else if (s.is_f16) *reinterpret_cast<uint2*>(a.out + y * D + d) = make_uint2(pack2<true>(u.x * f, u.y * f), pack2<true>(u.z * f, u.w * f));
+          else *reinterpret_cast<uint2*>(a.out + y * D + d) = make_uint2(pack2<false>(u.x * f, u.y * f), pack2<false>(u.z * f, u.w * f));
+        }
       }
       // O lay where the next copies go: order those writes before them.
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
