@@ -56,13 +56,24 @@ __device__ __forceinline__ int blocks_of(const SelectArgs& a, int t) {
 template <bool kF16>
 __global__ void __launch_bounds__(kScoreThreads) gqa_score_kernel(SelectArgs a) {
   __shared__ float warp_max[kScoreThreads / 32];
+  __shared__ int page_s[kScoreBlocks];
   __shared__ __align__(16) int8_t c8[256];
   const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   hk::let_next_grid_start();
   if (t >= a.cu[a.num_lanes]) return;
   const int n = blocks_of(a, t), from = blockIdx.z * kScoreBlocks, to = min(n - a.local, from + kScoreBlocks);
   if (n <= a.top || from >= to) return;
+  // The pages first: their addresses are what the loop waits for.
   const int b = hk::lane_of_row(a.cu, a.num_lanes, t);
+  for (int k = tid; k < kScoreBlocks; k += kScoreThreads) {
+    const int i = from + k;
+    int page = i < to && i < a.bt_stride ? a.bt[(int64_t)b * a.bt_stride + i] : -1;
+    if (page <= 0 || page >= a.num_pages) {
+      if (i < to && i >= a.sink) hk_flag(a.err, hk::kErrAttnPage, (unsigned)b);
+      page = -1;
+    }
+    page_s[k] = page;
+  }
   const int group = a.q_heads / a.kv_heads;
   float u[2] = {0.f, 0.f}, mine = 0.f;
 #pragma unroll
@@ -95,25 +106,20 @@ __global__ void __launch_bounds__(kScoreThreads) gqa_score_kernel(SelectArgs a) 
   }
   __syncthreads();
 
-  const int vec = a.dim / 16, sub = lane % vec;  // 4, 8 or 16 lanes per centroid
+  const int vec = a.dim / 16, sub = tid % vec;  // 4, 8 or 16 lanes per centroid
   const int4 y = reinterpret_cast<const int4*>(c8)[sub];
   uint32_t* keys = a.keys + ((int64_t)t * a.kv_heads + g) * a.max_blocks;
   const int per = kScoreThreads / vec;
-#pragma unroll 4
-  for (int base = from; base < to; base += per) {
-    const int i = base + tid / vec;
-    int page = -1;
-    if (i < to && i < a.bt_stride) page = a.bt[(int64_t)b * a.bt_stride + i];
-    const bool ok = page > 0 && page < a.num_pages;
+#pragma unroll 8
+  for (int base = 0; base < to - from; base += per) {
+    const int i = base + tid / vec, page = i < kScoreBlocks ? page_s[i] : -1;
+    const bool ok = page > 0;
     const int64_t at = (int64_t)(ok ? page : 0) * a.kv_heads + g;
     const int4 x = reinterpret_cast<const int4*>(a.centroids + at * a.dim)[sub];
     const float f = a.centroid_scale[at];
     int dot = __dp4a(x.x, y.x, __dp4a(x.y, y.y, __dp4a(x.z, y.z, __dp4a(x.w, y.w, 0))));
     for (int o = 1; o < vec; o <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (sub == 0 && i < to) {
-      if (!ok && i >= a.sink) hk_flag(a.err, hk::kErrAttnPage, (unsigned)b);
-      keys[i] = ok ? order_key(__fadd_rn(__fmul_rn((float)dot, f), 0.f)) : 0u;  // -0 becomes 0
-    }
+    if (sub == 0 && from + i < to) keys[from + i] = ok ? order_key(__fadd_rn(__fmul_rn((float)dot, f), 0.f)) : 0u;  // -0 becomes 0
   }
 }
 

@@ -7,11 +7,12 @@
 // (2i, 2i + 1) in the interleaved form; dims past rot pass unrotated.  Everything is fp32 from the
 // load to the one rounding of the store.
 //
-// Bound: HBM, each head read and written once.  A head is held by D / 8 lanes (rounded up to a
-// power of two), 16 bytes each, so the sum of squares is a few shuffles and the partner of a
-// rotated element is either in the same lane (interleaved) or rot / 16 lanes away.  A warp takes
-// kHeads heads of one row and issues all their loads first: that keeps enough bytes in flight, and the
-// row's cosines and sines are read once for all of them.
+// Bound: HBM, each head read and written once.  D / 8 lanes (rounded up to a power of two) hold a head, eight
+// elements each as two runs of four: four of the first half of the rotated dims and their four partners
+// (interleaved: eight neighbours), or eight dims past them.  So partners meet in one thread, and a lane's
+// products of gain with cosine and sine, the same for all heads, are formed once:
+//   out_j = (r x_j) A_j + (r x_p(j)) B_j,  A = gain * c,  B = -+ gain_p * s,  r = 1 / sqrt(mean + eps).
+// A warp takes kIters groups of heads of one row and issues all their loads first.
 #include "common.cuh"
 
 namespace {
@@ -28,7 +29,7 @@ struct NormRopeArgs {
   const float* table;
   int64_t table_rows;
   const int32_t* positions;
-  int32_t num_tokens, dim, rot, items;  // items: warps per row
+  int32_t num_tokens, dim, rot, items, q_items;  // warps per row, and those of q among them
   float eps;
   unsigned long long* err;
 };
@@ -48,76 +49,75 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(NormRopeArgs a) 
     if (lane == 0) hk_flag(a.err, hk::kErrPosition, (unsigned)t);
     return;
   }
-  const bool on = e0 < a.dim;
-  const int h0 = (int)(item - row * a.items) * (kGroups * kIters) + lane / LPH;
-  const int total = a.heads[0] + a.heads[1];
+  const int part = (int)(item - row * a.items);  // the first items of a row are of q, the others of k
+  const int w = part >= a.q_items;
+  const int heads = w ? a.heads[1] : a.heads[0];
+  const int h0 = (part - (w ? a.q_items : 0)) * (kGroups * kIters) + lane / LPH;
+  const int half = a.rot / 2;
+  const bool on = e0 < a.dim, turned = e0 < a.rot;
+  // This lane's two runs of four.
+  const int at0 = kPairs || !turned ? e0 : e0 / 2, at1 = kPairs || !turned ? e0 + 4 : half + e0 / 2;
+  const uint16_t* x = (w ? a.x[1] : a.x[0]) + t * (w ? a.xs[1] : a.xs[0]);
+  uint16_t* y = (w ? a.y[1] : a.y[0]) + t * (w ? a.ys[1] : a.ys[0]);
 
-  uint4 v[kIters];
+  uint2 v[kIters][2];
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
     const int h = h0 + i * kGroups;
-    v[i] = make_uint4(0, 0, 0, 0);
-    if (on && h < total) {
-      const int w = h >= a.heads[0];
-      v[i] = *reinterpret_cast<const uint4*>(a.x[w] + t * a.xs[w] + (int64_t)(h - w * a.heads[0]) * a.dim + e0);
+    v[i][0] = v[i][1] = make_uint2(0, 0);
+    if (on && h < heads) {
+      v[i][0] = *reinterpret_cast<const uint2*>(x + h * a.dim + at0);
+      v[i][1] = *reinterpret_cast<const uint2*>(x + h * a.dim + at1);
     }
   }
-  // This lane's 8 cosines and sines (4 of each, twice, when neighbours pair up); 1 and 0 outside the rotated dims.
-  float c[8], s[8];
-  const float* line = a.table + (int64_t)pos * a.rot;
-  const int half = a.rot / 2;
-  const bool turned = e0 < a.rot;
+  constexpr int kPartner = kPairs ? 1 : 4;
+  float A[8], B[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) c[j] = 1.f, s[j] = 0.f;
+  for (int j = 0; j < 8; ++j) A[j] = 1.f, B[j] = 0.f;
+  const uint16_t* gain = w ? a.gain[1] : a.gain[0];
+  if (gain != nullptr && on) {
+    const uint2 lo = *reinterpret_cast<const uint2*>(gain + at0), hi = *reinterpret_cast<const uint2*>(gain + at1);
+    unpack8<kF16>(make_uint4(lo.x, lo.y, hi.x, hi.y), A);
+  }
   if (turned) {
-    const float* f = line + (kPairs ? e0 / 2 : e0 < half ? e0 : e0 - half);
+    // Four angles: those of the first run (halves), or of the pairs (0, 1) (2, 3) (4, 5) (6, 7).
+    const float* line = a.table + (int64_t)pos * a.rot + e0 / 2;
+    const float4 cv = *reinterpret_cast<const float4*>(line), sv = *reinterpret_cast<const float4*>(line + half);
+    const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
 #pragma unroll
-    for (int j = 0; j < (kPairs ? 4 : 8); j += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(f + j), y = *reinterpret_cast<const float4*>(f + half + j);
-      const float cx[4] = {x.x, x.y, x.z, x.w}, sx[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (kPairs) c[2 * e] = c[2 * e + 1] = cx[e], s[2 * e] = s[2 * e + 1] = sx[e];
-        else c[j + e] = cx[e], s[j + e] = sx[e];
-      }
+    for (int j = 0; j < 8; ++j) {
+      const int f = kPairs ? j / 2 : j % 4;
+      B[j] = (j & kPartner) ? A[j ^ kPartner] * s[f] : -(A[j ^ kPartner] * s[f]);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) A[j] *= c[kPairs ? j / 2 : j % 4];
   }
   const float inv_dim = 1.f / (float)a.dim;
-  const int partner = e0 < half ? lane + half / 8 : lane - half / 8;  // halves form: rot % 16 == 0
-  const float sign = e0 < half ? -1.f : 1.f;
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
     const int h = h0 + i * kGroups;
-    const int w = h >= a.heads[0];
-    float x[8];
-    unpack8<kF16>(v[i], x);
+    float f[8];
+    unpack8<kF16>(make_uint4(v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y), f);
     float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+    for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float r = rsqrtf(fmaf(ss, inv_dim, a.eps));
     float g[8];
-    if (a.gain[w] != nullptr && on) {
-      unpack8<kF16>(*reinterpret_cast<const uint4*>(a.gain[w] + e0), g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * r * g[j];
-    } else {
+    for (int j = 0; j < 8; ++j) f[j] *= r;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= r;
+    for (int j = 0; j < 8; ++j) g[j] = f[j] * A[j];
+    if (turned) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = fmaf(f[j ^ kPartner], B[j], g[j]);
     }
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (kPairs) {
-        y[j] = (j & 1) ? fmaf(x[j], c[j], x[j ^ 1] * s[j]) : fmaf(x[j], c[j], -(x[j ^ 1] * s[j]));
-      } else {
-        const float other = __shfl_sync(0xffffffffu, x[j], turned ? partner : lane);
-        y[j] = turned ? fmaf(x[j], c[j], sign * (other * s[j])) : x[j];
-      }
+    if (on && h < heads) {
+      const uint4 u = pack8<kF16>(g);
+      *reinterpret_cast<uint2*>(y + h * a.dim + at0) = make_uint2(u.x, u.y);
+      *reinterpret_cast<uint2*>(y + h * a.dim + at1) = make_uint2(u.z, u.w);
     }
-    if (on && h < total)
-      *reinterpret_cast<uint4*>(a.y[w] + t * a.ys[w] + (int64_t)(h - w * a.heads[0]) * a.dim + e0) = pack8<kF16>(y);
   }
 }
 
@@ -164,7 +164,8 @@ extern "C" int hk_qk_norm_rope(const uint16_t* q, int64_t q_stride, const uint16
   a.num_tokens = num_tokens, a.dim = head_dim, a.rot = rot_dim, a.eps = eps, a.err = hk::err_word();
   const int lph = head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32;
   const int per = 32 / lph * kIters;
-  a.items = (q_heads + kv_heads + per - 1) / per;
+  a.q_items = (q_heads + per - 1) / per;
+  a.items = a.q_items + (kv_heads + per - 1) / per;
   const int64_t ctas = ((int64_t)num_tokens * a.items + kWarps - 1) / kWarps;
   HK_REQUIRE(ctas * kWarps <= INT32_MAX, "hk_qk_norm_rope: too many heads in one call");
   const cudaStream_t s = (cudaStream_t)stream;
