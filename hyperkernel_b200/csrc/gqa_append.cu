@@ -278,8 +278,8 @@ extern "C" int hk_gqa_append_fp8(const uint16_t* k_new, int64_t k_stride, const 
   a.cache[0] = k_cache, a.cache[1] = v_cache, a.scale[0] = k_scale, a.scale[1] = v_scale;
   a.slots = slot_mapping, a.num_tokens = num_tokens, a.heads = kv_heads, a.dim = head_dim, a.page_size = page_size;
   a.num_pages = num_pages, a.centroids = centroids, a.centroid_scale = centroid_scale, a.err = hk::err_word();
-  // Small calls: few rows to a CTA, for their latency (64 decode rows: 3.5 us at 8, 8 us at 32); large ones: fewer CTAs
-  // that find nothing to do.
+  // Small calls: few rows to a CTA, for their latency (64 decode rows: 4.3 us at 4, 16.4 us at 32); large ones: fewer CTAs
+  // that find nothing to do (5,800 rows of prompt chunks: 20.8 us at 32, 24.5 us at 16).
   const bool small = num_tokens <= 1024;
   const int rows = small ? 4 : 32;
   const int64_t ctas = ((int64_t)num_tokens + rows - 1) / rows * 2 * kv_heads;

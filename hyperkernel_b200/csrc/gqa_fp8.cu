@@ -42,9 +42,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = kWarps * 16;  // tokens
 constexpr int kMaxCtasPerSm = 5;
 
-// CTAs that an SM holds (by registers: 128 threads of at most 96, 128, 168 or 255).
+// CTAs that an SM holds (by registers: 128 threads of at most 96, 128, 168 or 255).  Three N tiles at dim 128 in 168
+// registers spill: 502 us against 472 us for 5 rows of 4 heads over a million tokens.
 constexpr int ctas_per_sm(int d, int nt) {
-  return d == 256 ? 2 : d * nt <= 64 ? 5 : d * nt <= 128 ? 4 : d * nt <= 384 ? 3 : 2;
+  return d == 256 ? 2 : d * nt <= 64 ? 5 : d * nt <= 128 ? 4 : d * nt <= 320 ? 3 : 2;
 }
 // Chunks a warp keeps in flight: what 200 KB of shared memory an SM hold.
 constexpr int stages(int d, int nt) { return 200 * 1024 / (ctas_per_sm(d, nt) * kWarps * 32 * d); }
@@ -232,11 +233,9 @@ struct State {
 };
 
 // S = K Q^T of one chunk: column n * 8 + 2c + (e & 1), token r + 8 (e >> 1).  q: this lane's B fragments, two k
-// steps to 16 bytes.  With one N tile the eight (dim 128) products are two chains, for their latency.
+// steps to 16 bytes.
 template <int D, int NT>
 __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&k)[2][D / 16], uint32_t q) {
-  constexpr int kChains = NT == 1 ? 2 : 1;
-  float acc[kChains][NT][4];
 #pragma unroll
   for (int i = 0; i < D / 16; i += 2) {
     uint32_t a[2][4];
@@ -248,16 +247,11 @@ __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&k)[2]
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const uint4 b = lds16(q + (n * (D / 32) + i / 2) * 512);
-      if (i == 0) mma_f16_first(acc[0][n], a[0][0], a[0][1], a[0][2], a[0][3], b.x, b.y);
-      else mma_f16(acc[0][n], a[0][0], a[0][1], a[0][2], a[0][3], b.x, b.y);
-      if (i == 0 && kChains == 2) mma_f16_first(acc[kChains - 1][n], a[1][0], a[1][1], a[1][2], a[1][3], b.z, b.w);
-      else mma_f16(acc[kChains - 1][n], a[1][0], a[1][1], a[1][2], a[1][3], b.z, b.w);
+      if (i == 0) mma_f16_first(s[n], a[0][0], a[0][1], a[0][2], a[0][3], b.x, b.y);
+      else mma_f16(s[n], a[0][0], a[0][1], a[0][2], a[0][3], b.x, b.y);
+      mma_f16(s[n], a[1][0], a[1][1], a[1][2], a[1][3], b.z, b.w);
     }
   }
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] = kChains == 2 ? acc[0][n][e] + acc[1][n][e] : acc[0][n][e];
 }
 
 // The scores of one chunk become weights (B fragments of P) and enter the running sums.  y: the chunk's
@@ -806,9 +800,10 @@ int n_tiles(int64_t rows, int dim) {
   return (int)(n < most ? n : most);
 }
 
-// Query rows (rows x heads of a group) of a lane above which the tcgen05 kernel takes it: two 32-row tiles of
-// the split kernel, which read the cache twice, against one of its 256-row tiles.
-constexpr int32_t kFewRows = 64;
+// Query rows (rows x heads of a group) of a lane above which the tcgen05 kernel takes it: above 32 the split kernel reads the
+// cache once for each 32 rows.  8 lanes of 20,000 tokens, 8 KV heads, 4 query heads each: 40 query rows 226 us (split) against
+// 204 us, 96 rows 317 against 208, 256 rows 768 against 249.
+constexpr int32_t kFewRows = 32;
 
 size_t split_workspace(int64_t rows, int dim);
 
