@@ -493,3 +493,78 @@ def test_wrappers_refuse_another_device_and_type(hk, cuda):
         hk.gqa_decode_fp8(q.transpose(1, 2).contiguous().transpose(1, 2), *four(c), bt, cu, pos, 1, b.max_kv, b.scale)
     with pytest.raises(hk.HKError):
         hk.gqa_decode_fp8(q, *four(c), bt, cu, pos, 1, b.max_kv, b.scale, workspace=torch.empty(16, dtype=torch.uint8, device=cuda))
+
+
+# ------------------------------------------------------------------------------------------
+# Batches wider than a CTA's scan, groups wider than a tile, lists longer than its registers
+# ------------------------------------------------------------------------------------------
+
+WIDE = {
+    "300 decode lanes": dict(rows=[1] * 300, ctx=[(37 * i) % 211 for i in range(300)], heads=4, kv=2, dim=64, page=32),
+    "idle lanes among 700, two chunks": dict(rows=[(0, 1, 0, 2)[i % 4] if i not in (513, 699) else 90 for i in range(700)], ctx=[(13 * i) % 90 for i in range(700)],
+                                             heads=2, kv=1, dim=64, page=16),
+    "64 heads to a group": dict(rows=[1, 3, 0, 1], ctx=[90, 20, 3, 400], heads=64, kv=1, dim=64, page=32),
+    "40 heads to a group, fp16": dict(rows=[2, 1], ctx=[300, 5], heads=80, kv=2, dim=128, page=64, dtype="f16"),
+    "20 wide heads to a group": dict(rows=[1, 2], ctx=[200, 40], heads=40, kv=2, dim=256, page=64),
+}
+
+
+@pytest.mark.parametrize("name", WIDE)
+def test_wide_batches(hk, cuda, name):
+    b = Batch(**WIDE[name], seed=len(name))
+    q, c, bt, cu, pos = on_gpu(b, cuda)
+    out, lse = hk.gqa_decode_fp8(q, *four(c), bt, cu, pos, b.max_rows, b.max_kv, b.scale)
+    hk.check_errors()
+    near(out, lse, b)
+    got = hk.gqa_select_blocks(q, c["cen"], c["cs"], bt, cu, pos, b.page, b.max_kv, 4, sink=1, local=1)
+    want = G8.select(b.q, b.cache, b.bt, b.cu, b.pos, 4, 1, 1)
+    assert np.array_equal(get(got), want)
+    out, lse = hk.gqa_sparse_fp8(q, *four(c), bt, cu, pos, got, b.scale)
+    hk.check_errors()
+    near(out, lse, b, blocks=want)
+
+
+@pytest.mark.parametrize("blocks", [4200, 17000])
+def test_long_lists_of_blocks(hk, cuda, blocks):
+    """More keys than 256 threads hold, and more than 1024 threads hold; equal scores among them."""
+    b = Batch([2], [blocks * 16 - 5], 2, 1, 64, 16, seed=blocks)
+    b.cache["cen"][1::7] = b.cache["cen"][1]
+    b.cache["cs"][1::7] = b.cache["cs"][1]
+    for top in (8, 300):
+        got, _ = _select(hk, b, cuda, top)
+        hk.check_errors()
+        assert np.array_equal(get(got), G8.select(b.q, b.cache, b.bt, b.cu, b.pos, top, 1, 2))
+
+
+@pytest.mark.parametrize("tokens", [3, 1500])
+def test_append_of_many_lanes(hk, cuda, tokens):
+    """Rows of many lanes, single ones and runs of all lengths around the limits of the short ones, in one call."""
+    rows = [1, 9, 8, 1, 70, 1, 17, 2] * (1 + tokens // 100)
+    ctx = [(29 * i) % 33 for i in range(len(rows))]
+    b = Batch(rows, ctx, 2, 2, 128, 32, seed=tokens)
+    k, v = b.new_rows()
+    want = {n: a.copy() for n, a in b.cache.items()}
+    G8.append(k, v, b.slots, want)
+    c = {n: put(a, cuda) for n, a in b.cache.items()}
+    hk.gqa_append_fp8(put(k, cuda, "bf16"), put(v, cuda, "bf16"), put(b.slots, cuda), *four(c), c["cen"], c["cs"])
+    hk.check_errors()
+    for name in ("ks", "vs", "k", "v", "cen", "cs"):
+        assert np.array_equal(get(c[name]), want[name], equal_nan=True), name
+
+
+def test_calls_on_two_streams_with_their_own_workspaces(hk, cuda):
+    """Two attentions at once give what each gives alone."""
+    cases = [Batch([1, 70, 3], [700, 90, 40], 8, 2, 128, 64, seed=30 + i) for i in range(2)]
+    on = [on_gpu(b, cuda) for b in cases]
+    alone = [hk.gqa_decode_fp8(q, *four(c), bt, cu, pos, b.max_rows, b.max_kv, b.scale) for b, (q, c, bt, cu, pos) in zip(cases, on)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[], []]
+    for _ in range(5):
+        for i, (b, (q, c, bt, cu, pos)) in enumerate(zip(cases, on)):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(hk.gqa_decode_fp8(q, *four(c), bt, cu, pos, b.max_rows, b.max_kv, b.scale))
+    torch.cuda.synchronize()
+    hk.check_errors()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i][0]) and torch.equal(l, alone[i][1]) for o, l in outs[i])
