@@ -8,8 +8,9 @@
 // head (rows of the lane x heads of the group) are the narrow side of the products, so the
 // tokens take the M side of mma.m16n8k16 and 8 x NT query rows the N side:
 //   S^T = K Q^T,  O^T += V^T P^T.
-// e4m3 is exact in fp16, and so is q once each row is scaled by a power of two, so the products are
-// those of the stored values; P is rounded to fp16 (2^-11, finer than the output's type).
+// e4m3 is exact in fp16, and so is q once each row is scaled by a power of two (but for values below 2^-21 of
+// the row's largest, which keep an absolute error of 2^-32 of it), so the products are those of the
+// stored values; P is rounded to fp16 (2^-11, no coarser than the output's type).
 //
 // Every warp streams 16-token chunks through a ring of its own in shared memory, filled by TMA (a chunk
 // of one page and head is contiguous: 16 * dim bytes), so bytes in flight cost no registers and
@@ -28,6 +29,10 @@
 // units of kWarps chunks, and every CTA takes an equal contiguous range of units.  Problems cut by
 // a range's end leave fp32 partials, two at most for each CTA, which gqa_merge_kernel joins in
 // the order of the ranges: results do not depend on timing.
+//
+// Measured: 64 lanes of 1K to 32K tokens, 64 query and 8 KV heads of 128: 215 us, 5.7 TB/s (88% of the measured copy rate); 5
+// rows of 32 heads over a million tokens: 468 us, 4.6 TB/s; one row over 778 tokens: 11 us, two launches and
+// their dependent loads.
 #include "common.cuh"
 #include "gqa_fp8.cuh"
 #include "sm100.cuh"

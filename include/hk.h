@@ -280,7 +280,8 @@ int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cach
  * so the lists do not depend on the batch.  A row whose u is not finite scores 0 everywhere.
  * Centroids are those of hk_gqa_append_fp8: every block but a row's last must be full.  Rows past
  * cu_seqlens[num_lanes] are left as they are; one past max_kv_len gets an empty list and sets the
- * device error word.  workspace: hk_gqa_select_workspace_size bytes, 16-byte aligned. */
+ * device error word.  max_kv_len holds at most 65,535 x 256 blocks.  workspace:
+ * hk_gqa_select_workspace_size bytes, 16-byte aligned. */
 size_t hk_gqa_select_workspace_size(int32_t num_tokens, int32_t kv_heads, int32_t page_size,
                                     int32_t max_kv_len);
 int hk_gqa_select_blocks(const uint16_t* q, int64_t q_stride, const int8_t* centroids,
