@@ -3,11 +3,16 @@
 The library is the product: every call below runs a CUDA kernel of libhk.so on the
 caller's stream.  There is no CPU fallback — if libhk.so is missing or the device is not an
 sm_100 part, calls raise HKError.  torch is used only for device memory and streams.
+
+With `stream=` a wrapper runs as under `torch.cuda.stream(stream)`: the outputs and scratch it allocates belong
+to that stream, so that their memory is not handed to another stream while the call's kernels use it.  As
+with every call on another stream, the caller orders the streams and keeps the inputs alive.
 """
 from __future__ import annotations
 
 import ctypes as C
 import functools
+import inspect
 import os
 import re
 from pathlib import Path
@@ -156,6 +161,26 @@ def stream_ptr(stream=None):
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())  # the current stream, without its Python object
 
 
+def _on_stream(fn):
+    """Runs a wrapper under the stream that it is given.  Its new outputs are the caller's current stream's to
+    read too: when they are freed, their memory waits for that stream as well."""
+    at = list(inspect.signature(fn).parameters).index("stream")
+
+    @functools.wraps(fn)
+    def on(*args, **kw):
+        stream = args[at] if len(args) > at else kw.get("stream")
+        if stream is None:
+            return fn(*args, **kw)
+        here = torch.cuda.current_stream(stream.device)
+        with torch.cuda.stream(stream):
+            out = fn(*args, **kw)
+        for t in out.values() if isinstance(out, dict) else out if isinstance(out, tuple) else (out,):
+            if t is not None:
+                t.record_stream(here)
+        return out
+    return on
+
+
 def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args))
 
@@ -189,6 +214,7 @@ def _u16(t):
 # Kernel wrappers (all tensors on the current CUDA device, contiguous)
 # ------------------------------------------------------------------------------------------
 
+@_on_stream
 def pack(lane_tokens, lane_pos, block_table, page_size, num_pages, max_tokens, stream=None):
     dev = lane_tokens.device
     L = lane_tokens.shape[0]
@@ -227,6 +253,7 @@ def kv_dequant_fp8_rows(kv_cache, kv_scale, slots, out, page_rows=64, stream=Non
     return out
 
 
+@_on_stream
 def kv_dequant_fp8(kv_cache, kv_scale, page_rows=64, out=None, pages=None, stream=None):
     """The FP8 cache [slots][576] as the page-blocked bf16 cache of hk_mla_decode (only the
     pages listed in `pages`, an int32 device tensor, when given)."""
@@ -245,6 +272,7 @@ def kv_append_f32(k_new, v_new, slot_mapping, k_cache, v_cache, stream=None):
          ptr(k_cache), ptr(v_cache), k_cache.shape[0], stream_ptr(stream))
 
 
+@_on_stream
 def gqa_decode(q, k_cache, v_cache, block_table, cu_seqlens, positions, kv_heads, page_size,
                scale, stream=None):
     T, qh, D = q.shape
@@ -260,6 +288,7 @@ def mla_workspace_size(num_lanes, num_tokens, heads, max_kv_len) -> int:
     return lib().hk_mla_workspace_size(num_lanes, num_tokens, heads, max_kv_len)
 
 
+@_on_stream
 def mla_decode(q, kv_cache, block_table, cu_seqlens, positions, page_size, max_kv_len, scale,
                out=None, lse=None, workspace=None, impl=0, stream=None):
     T, H, _ = q.shape
@@ -278,6 +307,7 @@ def mla_decode(q, kv_cache, block_table, cu_seqlens, positions, page_size, max_k
     return out, lse
 
 
+@_on_stream
 def mla_decode_fp8(q, kv_cache, kv_scale, block_table, cu_seqlens, positions, page_size,
                    max_kv_len, scale, stream=None):
     T, H, _ = q.shape
@@ -294,6 +324,7 @@ def mla_decode_fp8(q, kv_cache, kv_scale, block_table, cu_seqlens, positions, pa
     return out, lse
 
 
+@_on_stream
 def mla_partial_fp8(q, kv_cache, kv_scale, block_table, cu_seqlens, positions, kv_begin, kv_end,
                     page_size, max_kv_len, scale, stream=None):
     T, H, _ = q.shape
@@ -310,6 +341,7 @@ def mla_partial_fp8(q, kv_cache, kv_scale, block_table, cu_seqlens, positions, k
     return o, lse
 
 
+@_on_stream
 def mla_partial(q, kv_cache, block_table, cu_seqlens, positions, kv_begin, kv_end, page_size, max_kv_len,
                 scale, stream=None, out=None, lse=None):
     """Partial attention of KV ranges on the tcgen05 kernel over the page-blocked bf16 cache:
@@ -380,6 +412,7 @@ def _output(out, like, shape):
     return (out, *_rows(out))
 
 
+@_on_stream
 def qk_norm_rope(q, k, positions, table, q_gain=None, k_gain=None, interleaved=False, eps=1e-6,
                  q_out=None, k_out=None, stream=None):
     """RMS norm of each query and key head, then the rotation by table[positions] (fp32, the layout
@@ -464,6 +497,7 @@ def _lanes(block_table, cu_seqlens, positions, T):
             _typed(positions, _I32, "positions"))
 
 
+@_on_stream
 def gqa_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, max_rows,
                    max_kv_len, scale, out=None, lse=None, workspace=None, stream=None):
     """Ragged paged attention over the block-scaled cache of `gqa_append_fp8`: every lane's rows
@@ -479,6 +513,7 @@ def gqa_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlen
     return out, lse
 
 
+@_on_stream
 def gqa_select_blocks(q, centroids, centroid_scale, block_table, cu_seqlens, positions, page_size, max_kv_len,
                       top_blocks, sink=1, local=1, blocks=None, workspace=None, stream=None):
     """The blocks each row and KV head reads, by its int8 score against the pages' centroids:
@@ -502,6 +537,7 @@ def gqa_select_blocks(q, centroids, centroid_scale, block_table, cu_seqlens, pos
     return blocks
 
 
+@_on_stream
 def gqa_sparse_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, positions, blocks, scale,
                    out=None, lse=None, workspace=None, stream=None):
     """`gqa_decode_fp8` over the listed blocks of each row and KV head.  Returns (out, lse)."""
@@ -530,6 +566,7 @@ def sampling_array(samplings, device):
     return torch.from_numpy(a.view(np.uint8).copy()).to(device)
 
 
+@_on_stream
 def sample_verify(logits, cu_rows, sampling, state, drafts, block, n_logprobs, stream=None):
     """Draws and verifies every lane's rows: returns (ids [lanes, block], lp [lanes, block,
     2n+1]); `state` (uint64 stored as int64, one per lane) advances in place."""
@@ -546,6 +583,7 @@ def sample_verify(logits, cu_rows, sampling, state, drafts, block, n_logprobs, s
     return ids, lp
 
 
+@_on_stream
 def lse_merge(o_parts, lse_parts, stream=None):
     n, rows, dv = o_parts.shape
     out = torch.empty((rows, dv), dtype=torch.bfloat16, device=o_parts.device)
@@ -555,6 +593,7 @@ def lse_merge(o_parts, lse_parts, stream=None):
     return out, lse
 
 
+@_on_stream
 def quant_fp8(x, stream=None):
     rows, k = x.shape
     xq = torch.empty((rows, k), dtype=torch.uint8, device=x.device)
@@ -563,6 +602,7 @@ def quant_fp8(x, stream=None):
     return xq, sx
 
 
+@_on_stream
 def gemm_fp8(xq, sx, wq, sw, out=None, stream=None):
     m, k = xq.shape
     n = wq.shape[0]
@@ -572,6 +612,7 @@ def gemm_fp8(xq, sx, wq, sw, out=None, stream=None):
     return out
 
 
+@_on_stream
 def route(logits, bias, top_k, route_scale, stream=None):
     T, E = logits.shape
     ids = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
@@ -581,6 +622,7 @@ def route(logits, bias, top_k, route_scale, stream=None):
     return ids, w
 
 
+@_on_stream
 def permute(ids, weights, num_experts, stream=None, offsets=None, perm_token=None):
     """`offsets` / `perm_token` may be given as contiguous views of larger buffers (the first
     num_experts + 1 and T * K entries are written)."""
@@ -603,6 +645,7 @@ def moe_workspace_size(rows, hidden, inter) -> int:
     return lib().hk_moe_workspace_size(rows, hidden, inter)
 
 
+@_on_stream
 def moe_grouped(xq, sx, offsets, perm_token, rows, hidden, inter, w13, s13, w2, s2, out=None,
                 workspace=None, stream=None):
     E = offsets.shape[0] - 1
@@ -617,6 +660,7 @@ def moe_grouped(xq, sx, offsets, perm_token, rows, hidden, inter, w13, s13, w2, 
     return out
 
 
+@_on_stream
 def moe_grouped_noalloc(xq, sx, offsets, perm_token, rows, hidden, inter, w13, s13, w2, s2,
                         out=None, stream=None):
     """hk_moe_grouped with the library's fixed scratch array (no workspace argument)."""
@@ -629,6 +673,7 @@ def moe_grouped_noalloc(xq, sx, offsets, perm_token, rows, hidden, inter, w13, s
     return out
 
 
+@_on_stream
 def gather_rows(src, idx, out=None, stream=None):
     """out[i] = src[idx[i]] (rows of src as bytes; 16-byte multiples)."""
     rows = idx.shape[0]
@@ -647,6 +692,7 @@ def scatter_rows(src, idx, out, stream=None):
     return out
 
 
+@_on_stream
 def combine(y, perm_weight, inv, shared, tokens, top_k, out=None, stream=None):
     hidden = y.shape[1]
     if out is None:
