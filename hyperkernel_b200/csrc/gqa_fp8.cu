@@ -10,7 +10,7 @@
 //   S^T = K Q^T,  O^T += V^T P^T.
 // e4m3 is exact in fp16, and so is q once each row is scaled by a power of two (but for values below 2^-21 of
 // the row's largest, which keep an absolute error of 2^-32 of it), so the products are those of the
-// stored values; P is rounded to fp16 (2^-11, no coarser than the output's type).
+// stored values; P is rounded to fp16 (2^-11; below 2^-14 of 2^M to 2^-25 of it).
 //
 // Every warp streams 16-token chunks through a ring of its own in shared memory, filled by TMA (a chunk
 // of one page and head is contiguous: 16 * dim bytes), so bytes in flight cost no registers and
@@ -21,9 +21,9 @@
 // conversion, which makes the transposed fragment.  P^T reaches the layout of a B fragment by
 // movmatrix.
 //
-// With vs folded into the exponent, w_j = 2^(s_j + log2 vs - M), one running maximum M serves pages of
-// any scale, and sum_j w_j / vs is the softmax's denominator.  M is raised (and O rescaled) only when a
-// value passes it by more than 2^8, which fp16 weights have room for.
+// With vs folded into the exponent, w_j = 2^(s_j + log2 vs - M), one reference M serves pages of
+// any scale, and sum_j w_j / vs is the softmax's denominator.  M follows the row's largest weights (gqa_fp8.cuh); every
+// 16 chunks a warp looks whether it has to come down.
 //
 // Work split: the 16-token chunks of all (lane, KV head, row tile) problems lie end to end in
 // units of kWarps chunks, and every CTA takes an equal contiguous range of units.  Problems cut by
@@ -57,6 +57,7 @@ constexpr int stages(int d, int nt) { return 200 * 1024 / (ctas_per_sm(d, nt) * 
 constexpr int kLook = 16;           // chunks whose pages and scales are looked up at once
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+using hk::kNoMax;
 
 // What CTA i leaves for the merge: the problem its last range starts and does not finish, and whether the
 // problem it continues from the CTA before ends in it.
@@ -260,13 +261,12 @@ __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&k)[2]
 }
 
 // The scores of one chunk become weights (B fragments of P) and enter the running sums.  y: the chunk's
-// scales; `edge`: some token is past a row's position.  The running maximum starts at a finite
-// value far below any score, so that a masked score (-inf) weighs 0 with no further test.
-constexpr float kNoMax = -1e30f;
-
+// scales; `edge`: some token is past a row's position; `settle`: M may come down here.  M starts at a finite
+// value far below any score, so that a masked score (-inf) weighs 0 with no further test.  top_s: the highest M a
+// row has had.
 template <int D, int NT>
 __device__ __forceinline__ void weigh(State<D, NT>& st, float (&s)[NT][4], uint32_t (&b)[NT][2], const float (&rowf)[NT][2],
-                                      const Look& y, bool edge, const int* pos_s, int r, int c) {
+                                      const Look& y, bool edge, bool settle, const int* pos_s, float* top_s, int r, int c) {
   float p[NT][4];
   float most = -INFINITY;
 #pragma unroll
@@ -283,7 +283,19 @@ __device__ __forceinline__ void weigh(State<D, NT>& st, float (&s)[NT][4], uint3
     for (int e = 0; e < 4; ++e) p[n][e] = s[n][e] - st.m[n][e & 1];
     most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3])));
   }
-  if (__any_sync(0xffffffffu, most > 8.f)) {
+  if (settle) {  // does every row have a weight near M?
+    uint32_t near = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) near |= (uint32_t)(fmaxf(p[n][e], p[n][e + 2]) >= -hk::kSlack) << (2 * n + e);
+    if (__reduce_or_sync(0xffffffffu, near << (2 * NT * c)) != 0xffffffffu >> (32 - 8 * NT)) most = INFINITY;
+  }
+  if (__any_sync(0xffffffffu, most > hk::kRoom)) {
+    bool full = false;  // a sum that coming down could carry past fp32
+#pragma unroll
+    for (int n = 0; n < NT; ++n) full |= st.l[n][0] > hk::kFullSum || st.l[n][1] > hk::kFullSum;
+    settle = settle && !__any_sync(0xffffffffu, full);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -291,14 +303,19 @@ __device__ __forceinline__ void weigh(State<D, NT>& st, float (&s)[NT][4], uint3
         float t = fmaxf(s[n][e], s[n][e + 2]);
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
-        const float m = fmaxf(st.m[n][e], t);
+        const int row = n * 8 + 2 * c + e;
+        const float peak = top_s[row];
+        __syncwarp();
+        const float m = hk::new_reference(st.m[n][e], t, peak, settle);
+        if (r == 0) top_s[row] = fmaxf(peak, m);
+        p[n][e] = s[n][e] - m, p[n][e + 2] = s[n][e + 2] - m;
         const float f = exp2_approx(st.m[n][e] - m);
         st.m[n][e] = m;
         st.l[n][e] *= f;
-        p[n][e] = s[n][e] - m, p[n][e + 2] = s[n][e + 2] - m;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) st.o[j][n][e] *= f, st.o[j][n][e + 2] *= f;
       }
+    __syncwarp();
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -556,7 +573,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
         }
         if (lane == 0) rowf_s[n] = __uint_as_float((uint32_t)(127 - up) << 23);
       }
-      if (tid < R) pos_s[tid] = my_pos;
+      if (tid < R) {
+        pos_s[tid] = my_pos;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m_s[w][tid] = kNoMax;
+      }
       __syncthreads();
       float rowf[NT][2];
 #pragma unroll
@@ -575,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
 
 #pragma unroll 1
       for (int e = 0; e < nchunk; ++e) {
-        if (e > 0 && e % kLook == 0) look(e + kLook);
+        const bool again = e > 0 && e % kLook == 0;
+        if (again) look(e + kLook);
         ask(e + S - 1);  // into the stage that the step before has read
         if (line_s[warp][e % (2 * kLook)] < 0 || filled == 0) continue;
         const Look y = look_s[warp][e % (2 * kLook)];
@@ -590,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
             read_k<D>(k, mine, at);
             scores<D, NT>(sc, k, q_frag);
           }
-          weigh<D, NT>(st, sc, pb, rowf, y, edge, pos_s, r, c);
+          weigh<D, NT>(st, sc, pb, rowf, y, edge, again && !edge, pos_s, m_s[warp], r, c);
           uint32_t v[4][D / 32];
           read_v<D>(v, mine, at);
           if (edge) {  // tokens past the lane's end may hold anything, NaN codes among it

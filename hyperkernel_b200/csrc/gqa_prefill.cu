@@ -9,11 +9,11 @@
 //
 // e4m3 is exact in fp16, and so is q once each row is scaled by a power of two (but for values below 2^-21 of the
 // row's largest, which keep an absolute error of 2^-32 of it), so the products are those of the stored values.
-// P is rounded to fp16 (2^-11).  K and V come as e4m3 by TMA into a ring of 64-token stages, and four
+// P is rounded to fp16 (2^-11; below 2^-14 of 2^M to 2^-25 of it).  K and V come as e4m3 by TMA into a ring of 64-token stages, and four
 // warps convert them into the swizzled fp16 tiles the products read (a third of the softmax's instructions, as
 // 256 rows share it).  Scales of pages enter as one factor and one addend for each 16 tokens, and with log2 vs in
-// the exponent one running maximum serves pages of any scale (sum w / vs is the denominator).
-// M is raised, and O rescaled, only when a value passes it by more than 2^8.
+// the exponent one reference M serves pages of any scale (sum w / vs is the denominator).  M follows the row's largest
+// weights (gqa_fp8.cuh), step by step.
 //
 // Work split: the (row tile, head) problems' 128-token steps lie end to end, and every SM takes an
 // equal contiguous range of them.  Problems cut by a range's end leave fp32 partials, two at
@@ -42,7 +42,7 @@ constexpr int kStart = 2;     // what a problem costs besides its steps, in step
 constexpr int kParts = 4;     // a step's weights are handed over 32 tokens at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNoMax = -1e30f;
+using hk::kNoMax;
 // Registers: 512 threads x 128 = 2 x 128 x 184 (softmax) + 2 x 128 x 72 (the rest).
 constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
 
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       warp_arrive(bar(kQFull, half));
 
-      float m = kNoMax, l = 0.f;
+      float m = kNoMax, l = 0.f, peak = kNoMax;
       for (int i = first; i < last; ++i, ++n_s, ++step) {
         live = live && wait_bar(bar(kSFull, half), n_s & 1, abort, a.err, 0x70);
         live = __all_sync(0xffffffffu, live);
@@ -470,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
         }
         auto factor = [&](int k) { return kKeep ? f_kept[k & 1] : fmaxf(sc[k * (kBox / 16)].kf * rowf, 1.1754944e-38f); };  // above 0: a masked -inf stays one
         auto addend = [&](int k) { return kKeep ? lsv_kept[k & 1] : sc[k * (kBox / 16)].lsv; };
-        if ((i + 1) * kTok - 1 > pos_min) {
+        const bool edge = (i + 1) * kTok - 1 > pos_min;
+        if (edge) {
           const int seen = pos - i * kTok;  // tokens after it are masked
 #pragma unroll
           for (int e = 0; e < 128; ++e) v[e] = e > seen ? -INFINITY : v[e];
@@ -491,10 +492,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
           top = fmaxf(top, fmaf(most, factor(k), addend(k)));  // the factor is positive
         }
         // S is complete, so the product before it (which this row's O is from) is too.
-        const bool over = top > m + 8.f;
-        if (__any_sync(0xffffffffu, over)) {
-          const float m_new = over ? top : m, down = exp2_approx(m - m_new);
-          m = m_new;
+        if (__any_sync(0xffffffffu, top > m + hk::kRoom || (top < m - hk::kSlack && !edge))) {
+          const float m_new = hk::new_reference(m, top, peak, !edge && l < hk::kFullSum), down = exp2_approx(m - m_new);
+          m = m_new, peak = fmaxf(peak, m);
           l *= down;
           if (i > first) {
 #pragma unroll 1
