@@ -497,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
       const int32_t* list = kSparse ? a.blocks + ((int64_t)x.t0 * G + g) * a.top : nullptr;
       const int nchunk = tok1 > tok0 + 16 * warp ? (tok1 - tok0 - 16 * warp + kUnit - 1) / kUnit : 0;
       auto look = [&](int e0) {  // pages and scales of chunks e0 .. e0 + kLook - 1, a lane each
+        __syncwarp();  // every lane has read the places of the chunks before (skipped ones among them)
         if (lane < kLook && e0 + lane < nchunk) {
           int32_t line = -1;
           Look y = {0.f, 0.f, 1.f, 0};
