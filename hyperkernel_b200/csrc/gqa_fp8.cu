@@ -45,16 +45,26 @@ namespace sm100 = hk::sm100;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = kWarps * 16;  // tokens
-constexpr int kMaxCtasPerSm = 5;
+constexpr int kMaxCtasPerSm = 4;
 
-// CTAs that an SM holds (by registers: 128 threads of at most 96, 128, 168 or 255).  Three N tiles at dim 128 in 168
-// registers spill: 502 us against 472 us for 5 rows of 4 heads over a million tokens.
+// CTAs that an SM holds (by registers: 128 threads of at most 128, 168 or 255; by shared memory: see stages).  Three N tiles at
+// dim 128 in 168 registers spill: 502 us against 472 us for 5 rows of 4 heads over a million tokens.  Two and four N tiles at
+// dim 64 and four at dim 128 spill 4 to 60 bytes.  One N tile at dim 64 in five CTAs of 96 registers
+// and four stages: 132.0 us against 130.1 us for 64 lanes of 1K to 32K tokens, 32 query and 8 KV heads.
 constexpr int ctas_per_sm(int d, int nt) {
-  return d == 256 ? 2 : d * nt <= 64 ? 5 : d * nt <= 128 ? 4 : d * nt <= 320 ? 3 : 2;
+  return d == 256 ? 2 : d * nt <= 128 ? 4 : d * nt <= 320 ? 3 : 2;
 }
-// Chunks a warp keeps in flight: what 200 KB of shared memory an SM hold.
-constexpr int stages(int d, int nt) { return 200 * 1024 / (ctas_per_sm(d, nt) * kWarps * 32 * d); }
 constexpr int kLook = 16;           // chunks whose pages and scales are looked up at once
+// Shared memory of a CTA: the ring, up to 1 KB for its alignment, the fixed arrays (Q's fragments, the rows' sums, lookups and barriers),
+// and 1 KB that the device takes for itself; an SM has 228 KB.
+constexpr int kSmBytes = 228 * 1024, kCtaBytes = 1024, kAlignBytes = 1024;
+constexpr int fixed_bytes(int d, int nt) {
+  return 16 * nt * d + 8 * nt * (4 * (3 + 2 * kWarps) + 8) + kWarps * (2 * kLook * 20 + 8 * kLook + 16) + 64;
+}
+// Chunks a warp keeps in flight: what is left for the ring.
+constexpr int stages(int d, int nt) {
+  return (kSmBytes / ctas_per_sm(d, nt) - kCtaBytes - kAlignBytes - fixed_bytes(d, nt)) / (kWarps * 32 * d);
+}
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 using hk::kNoMax;
@@ -372,7 +382,7 @@ template <int D, int NT>
 constexpr int split_smem() {
   constexpr int ring = kWarps * stages(D, NT) * 32 * D, joined = kWarps * NT * (D / 16) * 32 * 16;  // O of every warp
   static_assert(stages(D, NT) >= 2 && stages(D, NT) <= kLook && joined <= ring, "ring");
-  return ring + 1024;  // lines are swizzled from 1 KB boundaries
+  return ring + kAlignBytes;  // lines are swizzled from 1 KB boundaries
 }
 
 template <int D, int NT, bool kSparse>
@@ -395,6 +405,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
   __shared__ __align__(8) uint64_t full_s[kWarps][S];
   __shared__ volatile int stop_s[kWarps];  // a wait of this warp ran out
   __shared__ __align__(16) Look look_s[kWarps][2 * kLook];
+  static_assert(sizeof q_s + sizeof rowf_s + sizeof m_s + sizeof l_s + sizeof pos_s + sizeof inv_s + sizeof row_s + sizeof scan_s + sizeof at_s +
+                        sizeof item_s + sizeof line_s + sizeof full_s + sizeof stop_s + sizeof look_s <= fixed_bytes(D, NT),
+                "fixed arrays");
+  static_assert(ctas_per_sm(D, NT) * (split_smem<D, NT>() + fixed_bytes(D, NT) + kCtaBytes) <= kSmBytes, "CTAs an SM holds");
   const GqaArgs& a = s.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int G = a.kv_heads, group = s.group;
@@ -842,8 +856,8 @@ int launch_one(SplitArgs& s, int64_t units, cudaStream_t stream) {
   constexpr int smem = split_smem<D, NT>();
   const int64_t resident = hk::sm_count() * ctas_per_sm(D, NT);
   const int grid = (int)(units < resident ? units : resident);
-  if (smem > 32 * 1024)  // set on every call: cheap, and right on every device
-    HK_TRY_CUDA(cudaFuncSetAttribute(gqa_split_kernel<D, NT, kSparse>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // (set on every call: cheap, and right on every device)
+  HK_TRY_CUDA(cudaFuncSetAttribute(gqa_split_kernel<D, NT, kSparse>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   CUtensorMap kmap, vmap;
   const uint64_t lines = (uint64_t)s.a.num_pages * s.a.kv_heads * s.a.page_size * D / 128;
   HK_REQUIRE(lines <= INT32_MAX, "the cache's K and V arrays must be below 2^38 bytes each");
