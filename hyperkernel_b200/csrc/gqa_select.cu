@@ -98,6 +98,11 @@ __global__ void __launch_bounds__(kScoreThreads) gqa_score_kernel(SelectArgs a) 
   float m = 0.f;
 #pragma unroll
   for (int w = 0; w < kScoreThreads / 32; ++w) m = fmaxf(m, warp_max[w]);
+  if (m < 0x1p-64f) {  // 127 / m could pass fp32: a power of two on u and m changes nothing else
+    m *= 0x1p64f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) u[k] *= 0x1p64f;
+  }
   // A row with a value that is not finite scores 0 everywhere.
   const float r = m > 0.f && m < INFINITY ? __fdiv_rn(127.f, m) : 0.f;
 #pragma unroll

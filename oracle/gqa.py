@@ -112,6 +112,8 @@ def select(q, cache, block_table, cu, positions, top, sink, local):
                 u = q[t].reshape(G, H // G, D)[g].astype(np.float64).sum(0).astype(np.float32)
                 m = np.abs(u).max()
                 c = np.zeros(D)
+                if m < 2.0 ** -64:  # 127 / m could pass fp32: a power of two changes nothing else
+                    u, m = u * np.float32(2.0 ** 64), m * np.float32(2.0 ** 64)
                 if m > 0 and np.isfinite(m):
                     c = np.rint(u * (np.float32(127) / m)).astype(np.float64)
                 pg = block_table[b, :n]

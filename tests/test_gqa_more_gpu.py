@@ -34,3 +34,21 @@ def test_skipped_chunks_where_lookups_meet(hk, cuda, page):
     with pytest.raises(hk.HKError, match="attn page"):
         hk.check_errors()
     near(out, lse, b)
+
+
+@pytest.mark.parametrize("down", [60, 100, 127])
+def test_selection_by_tiny_queries(hk, cuda, down):
+    """A power of two on a query changes none of its blocks, down to bf16's subnormals."""
+    b = Batch([1, 3], [3000, 1500], 8, 2, 128, 16, seed=51)
+    k = np.random.default_rng(52).integers(-64, 65, b.q.shape)
+    b.q = (k * 2.0 ** -3).astype(np.float32)
+    want = G8.select(b.q, b.cache, b.bt, b.cu, b.pos, 9, 1, 2)
+    q, c, bt, cu, pos = on_gpu(b, cuda)
+    small = put((k * 2.0 ** (-3 - down)).astype(np.float32), cuda, "bf16")
+    assert np.array_equal(get(small).astype(np.float64) * 2.0 ** (3 + down), k)  # nothing is lost in bf16
+    for x in (q, small):
+        got = hk.gqa_select_blocks(x, c["cen"], c["cs"], bt, cu, pos, 16, b.max_kv, 9, sink=1, local=2)
+        hk.check_errors()
+        assert np.array_equal(get(got), want)
+    b.q = (k * 2.0 ** (-3 - down)).astype(np.float32)
+    assert np.array_equal(G8.select(b.q, b.cache, b.bt, b.cu, b.pos, 9, 1, 2), want)
