@@ -35,7 +35,7 @@ struct GqaArgs {
 // below the range) costs the tokens after it nothing.  M does not come further than kDeep below its highest (there, fp16
 // reaches 2^-45 of the largest weight in full), nor where the sum is too large to be scaled.
 // (With M at the running maximum, the part of 30,000 tokens 17 nats below a first one was off by up to 3% of itself, and at 24 nats lost.)
-constexpr float kNoMax = -1e30f;
+constexpr float kNoMax = -3.402823466e38f;  // of a row that has seen no score: the lowest finite value
 constexpr float kHead = 7.f, kRoom = 15.f, kSlack = 3.f, kDeep = 16.f, kFullSum = 1e30f;
 
 __device__ __forceinline__ float new_reference(float m, float most, float peak, bool may_fall) {

@@ -52,3 +52,43 @@ def test_selection_by_tiny_queries(hk, cuda, down):
         assert np.array_equal(get(got), want)
     b.q = (k * 2.0 ** (-3 - down)).astype(np.float32)
     assert np.array_equal(G8.select(b.q, b.cache, b.bt, b.cu, b.pos, 9, 1, 2), want)
+
+
+@pytest.mark.parametrize("rows,ctx", [([1, 4], [50, 200])])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("size", [2.0 ** 30, 2.0 ** 97, 2.0 ** 101])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_scores_of_any_size(hk, cuda, rows, ctx, page, size, sign):
+    """Scores up to 1e34 and down to -1e34 weigh against each other as any others do; a row is empty only when it sees nothing."""
+    b = Batch(rows, ctx, 8, 2, 128, page, seed=53)
+    rng = np.random.default_rng(54)
+    pages = b.bt[b.bt > 0]
+    code = b.cache["k"][pages]
+    b.cache["k"][pages] = np.where(code == 0x7F, code, np.maximum(code & 0x7F, 0x38))  # keys at least 1 in every dim
+    b.cache["ks"][pages] = 1
+    b.q = rounded(sign * np.abs(rng.standard_normal(b.q.shape)).astype(np.float32) * np.float32(size), "bf16")
+    q, c, bt, cu, pos = on_gpu(b, cuda)
+    out, lse = hk.gqa_decode_fp8(q, *four(c), bt, cu, pos, b.max_rows, b.max_kv, b.scale)
+    hk.check_errors()
+    want, wl, mag, _ = G8.attend(b.q, b.cache, b.bt, b.cu, b.pos, b.scale)
+    # A score is off by 2^-20 of its size at most, far more than 1: which of two tokens that near each other has the weight is
+    # open, all others have none.  So rows whose two largest scores are further apart are that of one token, the others finite.
+    assert np.isfinite(get(out)).all()
+    assert (np.abs(get(lse).astype(np.float64) - wl) <= 2.0 ** -18 * np.abs(wl)).all()
+    second = second_scores(b)
+    clear = wl - second > 2.0 ** -17 * np.abs(wl)
+    assert clear.mean() > 0.9
+    assert (np.abs(get(out) - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * mag)[clear].all()
+
+
+def second_scores(b):
+    """The second largest score of each row and head (-inf: none)."""
+    out = np.full((b.T, b.heads), -np.inf)
+    for lane in range(len(b.rows)):
+        for t in range(b.cu[lane], b.cu[lane + 1]):
+            i = np.arange(b.pos[t] + 1)
+            k = G8.E4M3[b.cache["k"][b.bt[lane, i // b.page], :, i % b.page]].transpose(1, 0, 2)  # ks is 1
+            s = np.einsum("ghd,gnd->ghn", b.q[t].reshape(b.kv, -1, b.dim).astype(np.float64), k).reshape(b.heads, -1) * b.scale
+            if len(i) > 1:
+                out[t] = np.sort(s, -1)[:, -2]
+    return out
