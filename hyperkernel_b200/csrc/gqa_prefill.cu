@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       warp_arrive(bar(kQFull, half));
 
-      float m = kNoMax, l = 0.f, peak = kNoMax;
+      float m = kNoMax, l = 0.f, peak = kNoMax, soft = 1.f, soft_m = kNoMax;
       for (int i = first; i < last; ++i, ++n_s, ++step) {
         live = live && wait_bar(bar(kSFull, half), n_s & 1, abort, a.err, 0x70);
         live = __all_sync(0xffffffffu, live);
@@ -495,6 +495,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
         if (__any_sync(0xffffffffu, top > m + hk::kRoom || (top < m - hk::kSlack && !edge))) {
           const float m_new = hk::new_reference(m, top, peak, !edge && l < hk::kFullSum), down = exp2_approx(m - m_new);
           m = m_new, peak = fmaxf(peak, m);
+          // A weight's exponent is one fused product and sum, M a rounded one: from 2^26 on their difference could pass fp16's room.  Scores
+          // of that size are good to 2^-20 of it, so distances from M are taken in units of 2^-24 of it.
+          const uint32_t size = __float_as_uint(m) >> 23 & 255;
+          soft = size < 127 + 26 ? 1.f : __uint_as_float((127 + 24 + 127 - size) << 23);
+          soft_m = m * soft;
           l *= down;
           if (i > first) {
 #pragma unroll 1
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const int t = 32 * j + e, k = t / kBox;
-            const float f = factor(k), c = addend(k) - m;
+            const float f = factor(k) * soft, c = fmaf(addend(k), soft, -soft_m);
             const uint64_t x = fma2(pair(v[t], v[t + 1]), pair(f, f), pair(c, c));
             float x0, x1;
             unpair(x, x0, x1);

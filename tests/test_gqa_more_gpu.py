@@ -54,7 +54,7 @@ def test_selection_by_tiny_queries(hk, cuda, down):
     assert np.array_equal(G8.select(b.q, b.cache, b.bt, b.cu, b.pos, 9, 1, 2), want)
 
 
-@pytest.mark.parametrize("rows,ctx", [([1, 4], [50, 200])])
+@pytest.mark.parametrize("rows,ctx", [([1, 4], [50, 200]), ([1, 40], [50, 20]), ([140], [700])])
 @pytest.mark.parametrize("page", [16, 32, 64])
 @pytest.mark.parametrize("size", [2.0 ** 30, 2.0 ** 97, 2.0 ** 101])
 @pytest.mark.parametrize("sign", [-1, 1])
