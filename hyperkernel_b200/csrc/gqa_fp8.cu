@@ -509,6 +509,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
       // This warp's chunks: tokens tok0 + 16 warp + kUnit e.
       const int32_t* row_bt = a.bt + (int64_t)lane_b * a.bt_stride;
       const int32_t* list = kSparse ? a.blocks + ((int64_t)x.t0 * G + g) * a.top : nullptr;
+      if (kSparse && first == 0 && x.len > 0) {  // nothing may stand behind as many entries as blocks are in sight
+        for (int e = x.len / a.page_size + tid; e < a.top; e += kThreads)
+          if (list[e] != -1) hk_flag(a.err, hk::kErrBlockList, (unsigned)x.t0);
+      }
       const int nchunk = tok1 > tok0 + 16 * warp ? (tok1 - tok0 - 16 * warp + kUnit - 1) / kUnit : 0;
       auto look = [&](int e0) {  // pages and scales of chunks e0 .. e0 + kLook - 1, a lane each
         __syncwarp();  // every lane has read the places of the chunks before (skipped ones among them)

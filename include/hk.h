@@ -296,8 +296,9 @@ int hk_gqa_select_blocks(const uint16_t* q, int64_t q_stride, const int8_t* cent
 /* hk_gqa_decode_fp8 restricted, for each row and KV head, to the listed blocks (rising block
  * indices, -1 behind the last; hk_gqa_select_blocks writes them).  An index that does not rise above
  * the entry before it, follows a -1 or lies past the row's position is skipped and sets the device
- * error word.  An empty list gives
- * out 0 and lse -inf. */
+ * error word (each is compared with the one before it alone: an index that comes again behind one
+ * that was skipped counts again).  An empty list gives out 0 and lse -inf; the list of a row with a
+ * negative position is not read.  top_blocks: 1 to 4,096. */
 int hk_gqa_sparse_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache,
                       const uint8_t* v_cache, const float* k_scale, const float* v_scale,
                       const int32_t* block_table, int32_t bt_stride, const int32_t* cu_seqlens,

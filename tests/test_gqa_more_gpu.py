@@ -92,3 +92,31 @@ def second_scores(b):
             if len(i) > 1:
                 out[t] = np.sort(s, -1)[:, -2]
     return out
+
+
+@pytest.mark.parametrize("tail", [[5], [-1, 1], [-1, -1, 7], [-2], [1 << 30]])
+def test_entries_behind_the_blocks_in_sight_are_reported(hk, cuda, tail):
+    """A list as long as what is in sight, or shorter, and behind it entries that no row may read."""
+    b = Batch([1, 2], [40, 20], 4, 2, 64, 32, seed=55)  # 2 blocks in sight of the first row, 1 of the others
+    q, c, bt, cu, pos = on_gpu(b, cuda)
+    lists = np.full((3, 2, 8), -1, np.int32)
+    lists[0, :, :2], lists[1:, :, 0] = [0, 1], 0
+    out, lse = hk.gqa_sparse_fp8(q, *four(c), bt, cu, pos, put(lists, cuda), b.scale)
+    hk.check_errors()
+    near(out, lse, b, blocks=lists)
+    for t, g in ((0, 1), (2, 0)):
+        bad = lists.copy()
+        at = 2 if t == 0 else 1
+        bad[t, g, at:at + len(tail)] = tail
+        again = hk.gqa_sparse_fp8(q, *four(c), bt, cu, pos, put(bad, cuda), b.scale)
+        with pytest.raises(hk.HKError, match="block list"):
+            hk.check_errors()
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    # the list of a row that sees nothing is not read
+    p = b.pos.copy()
+    p[0] = -1
+    bad = lists.copy()
+    bad[0] = 99
+    out, lse = hk.gqa_sparse_fp8(q, *four(c), bt, cu, put(p, cuda), put(bad, cuda), b.scale)
+    hk.check_errors()
+    near(out, lse, b, blocks=lists, pos=p)
