@@ -728,6 +728,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) gqa_split_kernel
     }
   }
   if (tid == 0) s.rec[blockIdx.x] = rec;
+  if (dead) {  // a wait has run out: copies still in flight get time to land before the CTA ends
+    const unsigned long long t0 = sm100::globaltimer();
+    while (sm100::globaltimer() - t0 < 100000000ull) {
+    }
+  }
 }
 
 // Joins the partials of the problems that CTAs of the split kernel began and left open (their records), row blockIdx.y of

@@ -757,6 +757,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_prefill_kernel(PrefillArgs s,
     }
   }
   __syncthreads();
+  if (*abort) {  // a wait has run out: copies still in flight get time to land before the CTA ends
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 100000000ull) {
+    }
+  }
   if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
