@@ -158,7 +158,10 @@ def ptr(t):
 def stream_ptr(stream=None):
     if stream is not None:
         return stream.cuda_stream
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())  # the current stream, without its Python object
+    try:
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())  # the current stream, without its Python object
+    except AttributeError:  # not a public name of torch
+        return torch.cuda.current_stream().cuda_stream
 
 
 def _on_stream(fn):

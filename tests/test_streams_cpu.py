@@ -104,3 +104,10 @@ def test_what_a_call_allocates_belongs_to_its_stream(hk, watched, name, how):
 def test_every_wrapper_with_a_stream_is_looked_at(hk):
     with_stream = {n for n, f in inspect.getmembers(hk, inspect.isfunction) if "stream" in inspect.signature(f).parameters and not n.startswith("_")}
     assert with_stream == set(CALLS) | WRITES_INTO_ITS_ARGUMENTS
+
+
+def test_the_current_stream_without_torchs_private_name(hk, monkeypatch):
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: HERE)
+    assert hk.stream_ptr() == HERE.cuda_stream and hk.stream_ptr(FakeStream(5)) == 5
