@@ -30,9 +30,9 @@
 // a range's end leave fp32 partials, two at most for each CTA, which gqa_merge_kernel joins in
 // the order of the ranges: results do not depend on timing.
 //
-// Measured: 64 lanes of 1K to 32K tokens, 64 query and 8 KV heads of 128: 215 us, 5.7 TB/s (88% of the measured copy rate); 5
-// rows of 32 heads over a million tokens: 468 us, 4.6 TB/s; one row over 778 tokens: 11 us, two launches and
-// their dependent loads.
+// Measured: 64 lanes of 1K to 32K tokens, 64 query and 8 KV heads of 128: 217 us, 5.6 TB/s (87% of the measured copy rate); 32
+// query and 8 KV heads of 64: 132 us, 4.6 TB/s; 5 rows of 32 heads over a million tokens: 474 us, 4.5 TB/s; one
+// row over 778 tokens: 11 us, two launches and their dependent loads.
 #include "common.cuh"
 #include "gqa_fp8.cuh"
 #include "sm100.cuh"
@@ -48,7 +48,7 @@ constexpr int kUnit = kWarps * 16;  // tokens
 constexpr int kMaxCtasPerSm = 4;
 
 // CTAs that an SM holds (by registers: 128 threads of at most 128, 168 or 255; by shared memory: see stages).  Three N tiles at
-// dim 128 in 168 registers spill: 502 us against 472 us for 5 rows of 4 heads over a million tokens.  Two and four N tiles at
+// dim 128 in 168 registers spill: 481 us against 474 us for 5 rows of 4 heads over a million tokens.  Two and four N tiles at
 // dim 64 and four at dim 128 spill 4 to 60 bytes.  One N tile at dim 64 in five CTAs of 96 registers
 // and four stages: 132.0 us against 130.1 us for 64 lanes of 1K to 32K tokens, 32 query and 8 KV heads.
 constexpr int ctas_per_sm(int d, int nt) {
@@ -852,8 +852,8 @@ int n_tiles(int64_t rows, int dim) {
 }
 
 // Query rows (rows x heads of a group) of a lane above which the tcgen05 kernel takes it: above 32 the split kernel reads the
-// cache once for each 32 rows.  8 lanes of 20,000 tokens, 8 KV heads, 4 query heads each: 40 query rows 226 us (split) against
-// 204 us, 96 rows 317 against 208, 256 rows 768 against 249.
+// cache once for each 32 rows.  8 lanes of 20,000 tokens, 8 KV heads, 4 query heads each: 40 query rows 216 us (split) against
+// 176 us, 96 rows 312 against 180, 256 rows 796 against 213.
 constexpr int32_t kFewRows = 32;
 
 size_t split_workspace(int64_t rows, int dim);

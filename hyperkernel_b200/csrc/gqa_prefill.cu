@@ -20,8 +20,8 @@
 // most for each SM, which the merge kernel joins in the order of the ranges.
 //
 // Bound by the softmax and the products it waits for in turn.  Measured, 32 query and 8 KV heads of 128: 2048 rows behind
-// 30,000 tokens 1.10 ms, 947 TFLOP/s (56% of the measured bf16 burst rate); four chunks of 512 to 2048 rows behind
-// 1,000 to 6,000 tokens 456 us, 706 TFLOP/s.
+// 30,000 tokens 1.08 ms, 960 TFLOP/s (56% of the measured bf16 burst rate); four chunks of 512 to 2048 rows behind
+// 1,000 to 6,000 tokens 459 us, 701 TFLOP/s.
 //
 // Roles (16 warps): 0-3 and 4-7 softmax of the two halves, 8-11 conversion, 12 and 14 product issue of the
 // halves, 13 TMA.

@@ -13,7 +13,7 @@
 // products of gain with cosine and sine, the same for all heads, are formed once:
 //   out_j = (r x_j) A_j + (r x_p(j)) B_j,  A = gain * c,  B = -+ gain_p * s,  r = 1 / sqrt(mean + eps).
 // A warp takes kIters groups of heads of one row and issues all their loads first.  Measured: 8192 rows of 64 + 8 heads of
-// 128, 58.5 us, 5.2 TB/s (81% of the measured copy rate); 64 rows 2.7 us.
+// 128, 59.7 us, 5.1 TB/s (80% of the measured copy rate); 64 rows 2.8 us.
 #include "common.cuh"
 
 namespace {

@@ -239,7 +239,8 @@ int hk_qk_norm_rope(const uint16_t* q, int64_t q_stride, const uint16_t* k, int6
  * the pool, or a row of the run's page that does not take the slot after the row before it (the
  * same slot twice, a gap), is skipped and sets the device error word.  A value that is not
  * finite sets the error word, does not count in max|x|, and is stored as +-448 (infinities) or 0
- * (NaN), so a page never holds a NaN code.  Two runs in one call on the same page are a caller's
+ * (NaN), so a page never holds a NaN code.  Rows that follow a skipped one in its page are skipped
+ * with it.  Two runs in one call on the same page are a caller's
  * error: they write it at the same time, and its rows and scale are then unspecified.
  * head_dim 64, 128 or 256; page_size a multiple of 16 up to 256; strides in elements. */
 int hk_gqa_append_fp8(const uint16_t* k_new, int64_t k_stride, const uint16_t* v_new,
@@ -248,17 +249,22 @@ int hk_gqa_append_fp8(const uint16_t* k_new, int64_t k_stride, const uint16_t* v
                       int64_t num_pages, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
                       float* v_scale, int8_t* centroids, float* centroid_scale, void* stream);
 
-/* Attention over the block-scaled cache (any positive finite scales, not only powers of two):
+/* Attention over the block-scaled cache (any positive finite scales, not only powers of two; a V
+ * scale below 2^-100 counts as 2^-100):
  * query row t of lane b sits at positions[t] and attends rows 0..positions[t] of the lane.
  * q[T][q_heads][head_dim] (rows q_stride elements apart), out[T][q_heads][head_dim] of the same
  * type, lse[T][q_heads] (natural log, of scale * q.k); q_heads a multiple of kv_heads, query head
  * h reads KV head h / (q_heads / kv_heads).  Rows at and past cu_seqlens[num_lanes] are left as
  * they are; a row with a negative position gets out 0 and lse -inf.  Positions of a lane rise by
- * one.  max_rows and max_kv_len bound a lane's rows and KV rows (they choose the kernel and the
- * grid); a lane past max_rows is skipped and sets the device error word, as a page that is
- * 0 or past the pool does (its rows are not attended).  Cache rows past a lane's last position may
- * hold anything.  A NaN code in an attended V row reaches every row of that lane in this call.
- * workspace: hk_gqa_fp8_workspace_size bytes, 256-byte aligned. */
+ * one (negative ones too).  max_rows and max_kv_len bound a lane's rows and KV rows (they choose the
+ * kernel and the grid); a lane past max_rows is skipped and sets the device error word, as a page
+ * that is 0 or past the pool does (its rows are not attended).  Cache rows past a lane's last
+ * position may hold anything.  A NaN code in an attended V row reaches every row of that lane in this
+ * call.  head_dim 64, 128 or 256; page_size a multiple of 16 up to 256; scale positive and finite;
+ * k_cache and v_cache below 2^38 bytes each.  Computed in fp32 but for two roundings to fp16: of a query
+ * row scaled by a power of two (exact but for values below 2^-21 of the row's largest), and of the
+ * softmax's weights (2^-11 of each; small ones 2^-22 of the largest among some 256 tokens around
+ * them).  workspace: hk_gqa_fp8_workspace_size bytes, 256-byte aligned. */
 size_t hk_gqa_fp8_workspace_size(int32_t num_tokens, int32_t q_heads, int32_t kv_heads,
                                  int32_t head_dim);
 int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cache,
@@ -280,7 +286,8 @@ int hk_gqa_decode_fp8(const uint16_t* q, int64_t q_stride, const uint8_t* k_cach
  * so the lists do not depend on the batch.  A row whose u is not finite scores 0 everywhere.
  * Centroids are those of hk_gqa_append_fp8: every block but a row's last must be full.  Rows past
  * cu_seqlens[num_lanes] are left as they are; one past max_kv_len gets an empty list and sets the
- * device error word.  max_kv_len holds at most 65,535 x 256 blocks.  workspace:
+ * device error word.  head_dim 64, 128 or 256; page_size a multiple of 16 up to 256; top_blocks 1 to
+ * 4,096, of which sink + local at most; max_kv_len holds at most 65,535 x 256 blocks.  workspace:
  * hk_gqa_select_workspace_size bytes, 16-byte aligned. */
 size_t hk_gqa_select_workspace_size(int32_t num_tokens, int32_t kv_heads, int32_t page_size,
                                     int32_t max_kv_len);
