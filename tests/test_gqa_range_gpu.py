@@ -53,8 +53,8 @@ def long_lane(rows, ctx, dim, peaks, dtype="f16", equal=False, sink_v=0.0, heads
     return b
 
 
-def check(hk, cuda, b, blocks=None, ratio=1.0, lanes=1):
-    """The lane `lanes` times over, so that a CTA walks whole lanes."""
+def check(hk, cuda, b, blocks=None, ratio=1.0, lanes=1, unit=1.0):
+    """The lane `lanes` times over, so that a CTA walks whole lanes; outputs in units of `unit`, a power of two."""
     c = {n: put(x, cuda) for n, x in b.cache.items()}
     q = put(b.q, cuda).to(TORCH[b.dtype]).repeat(lanes, 1, 1)
     cu = np.arange(lanes + 1, dtype=np.int32) * b.T
@@ -66,9 +66,10 @@ def check(hk, cuda, b, blocks=None, ratio=1.0, lanes=1):
     hk.check_errors()
     want, wl, mag, size = G8.attend(b.q, b.cache, b.bt, b.cu, b.pos, b.scale, blocks)
     ds = (2.0 ** -20 * size)[..., None]
+    want, mag = want / unit, mag / unit
     peak = 2.0 ** -32 * b.window * ratio
     tol = HALF_STEP[b.dtype] * np.abs(want) + (2.0 ** -11 + 2.0 ** -14 + 2 * ds) * mag + peak + 2.0 ** -25
-    off = np.abs(out.float().cpu().numpy().astype(np.float64).reshape(lanes, *want.shape) - want) / tol
+    off = np.abs(out.float().cpu().numpy().astype(np.float64).reshape(lanes, *want.shape) / unit - want) / tol
     assert off.max() <= 1, f"{(off > 1).sum()} of {off.size} off, worst {off.max():.2f} of the tolerance (outputs up to {np.abs(want).max():.2e})"
     assert (np.abs(lse.cpu().numpy().reshape(lanes, *wl.shape) - wl) <= ds[..., 0] + 2.0 ** -20 * (1 + np.abs(wl))).all()
 
@@ -123,3 +124,11 @@ def test_a_page_with_a_large_value_scale(hk, cuda, rows, up):
     b.cache["vs"][b.bt[0, 100]] = 2.0 ** (up - 1)
     # one token's weight here is at most e^6 of the mean of 30,000
     check(hk, cuda, b, ratio=2.0 ** up * np.exp(6) / 30000)
+
+
+@pytest.mark.parametrize("rows", [1, 20], ids=["row", "chunk"])
+@pytest.mark.parametrize("peaks,unit", [({0: 20.0}, 2.0 ** -40), ({0: 20.0}, 2.0 ** 60), ({}, 2.0 ** -98), ({}, 2.0 ** 100)])
+def test_value_scales_of_any_size(hk, cuda, rows, peaks, unit):
+    b = long_lane(rows, 30000, 128, peaks, dtype="bf16", seed=12)
+    b.cache["vs"][:] *= np.float32(unit)
+    check(hk, cuda, b, unit=unit)

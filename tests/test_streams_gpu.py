@@ -62,3 +62,29 @@ def test_mla_calls_on_a_given_stream(hk, cuda):
     cu, pos = put(np.array([0, 2], np.int32), cuda), put(np.array([kv - 2, kv - 1], np.int32), cuda)
     ws = hk.mla_workspace_size(1, 2, heads, kv)
     queued_behind_other_work(hk, lambda s: hk.mla_decode(q, cache, bt, cu, pos, page, kv, 0.05, stream=s), ws)
+
+
+def test_a_call_on_a_given_stream_is_captured(hk, cuda):
+    b = Batch([1, 3], [700, 300], 8, 2, 128, 32, seed=41)
+    c = {n: put(a, cuda) for n, a in b.cache.items()}
+    q, bt, cu, pos = put(b.q, cuda).to(torch.bfloat16), put(b.bt, cuda), put(b.cu, cuda), put(b.pos, cuda)
+    call = lambda s: hk.gqa_decode_fp8(q, c["k"], c["v"], c["ks"], c["vs"], bt, cu, pos, b.max_rows, b.max_kv, b.scale, stream=s)
+    alone = call(None)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        here = torch.cuda.current_stream()
+        first = call(here)  # the capture's own stream, and one forked from it
+        other.wait_stream(here)
+        second = call(other)
+        here.wait_stream(other)
+        both = [torch.cat([u, w]) for u, w in zip(first, second)]
+        del first, second
+        third = call(here)
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    hk.check_errors()
+    for u, w, x in zip(alone, both, third):
+        assert torch.equal(torch.cat([u, u]), w) and torch.equal(u, x)
